@@ -52,8 +52,39 @@ EXPORTS = (
     "actune_selftest_wait_timeout",
 )
 
+# Symbols of actune_b200_serving.h.
+SERVING_EXPORTS = (
+    "actune_gated_norm",
+    "actune_adapter_plan_size",
+    "actune_adapter_plan",
+    "actune_adapter_workspace_size",
+    "actune_adapter_add",
+)
+
 _LIB = None
 _LOCK = threading.Lock()
+
+
+class GatedNormArgs(ctypes.Structure):
+    """actune_gated_norm_args (include/actune_b200_serving.h)."""
+
+    _fields_ = ([("struct_bytes", ctypes.c_size_t)]
+                + [(n, ctypes.c_void_p) for n in ("x", "residual", "post_weight", "pre_weight", "gate", "shift", "out",
+                                                  "residual_out", "packed", "scales")]
+                + [(n, ctypes.c_int64) for n in ("T", "D", "x_stride", "residual_stride", "post_rows", "pre_rows",
+                                                 "gate_rows", "shift_rows")]
+                + [("residual_scale", ctypes.c_float), ("eps", ctypes.c_float)]
+                + [(n, ctypes.c_int32) for n in ("dtype", "gemma", "quant_bits", "codes8")])
+
+
+class AdapterArgs(ctypes.Structure):
+    """actune_adapter_args (include/actune_b200_serving.h)."""
+
+    _fields_ = ([("struct_bytes", ctypes.c_size_t)]
+                + [(n, ctypes.c_void_p) for n in ("x", "y", "down", "up", "scale", "plan", "out", "workspace")]
+                + [("workspace_bytes", ctypes.c_size_t)]
+                + [(n, ctypes.c_int64) for n in ("M", "N", "K", "S", "R", "x_stride", "y_stride", "out_stride")]
+                + [(n, ctypes.c_int32) for n in ("tile", "dtype")])
 
 
 class ActuneError(RuntimeError):
@@ -89,8 +120,15 @@ def _declare(L):
     L.actune_set_wait_limit_ns.argtypes = [ctypes.c_uint64]
     L.actune_wait_limit_ns.argtypes = [ctypes.POINTER(ctypes.c_uint64)]
     L.actune_selftest_wait_timeout.argtypes = [i32, p]
-    for name in EXPORTS:
-        if name not in ("actune_status_string", "actune_grouped_linear_workspace_size"):
+    L.actune_gated_norm.argtypes = [ctypes.POINTER(GatedNormArgs), p]
+    L.actune_adapter_plan_size.argtypes = [i64, i64, i32]
+    L.actune_adapter_plan.argtypes = [p, i64, i64, i32, p, p]
+    L.actune_adapter_workspace_size.argtypes = [i64, i64, i64, i64, i32]
+    L.actune_adapter_add.argtypes = [ctypes.POINTER(AdapterArgs), p]
+    for name in EXPORTS + SERVING_EXPORTS:
+        if name.endswith("_size"):
+            getattr(L, name).restype = sz
+        elif name != "actune_status_string":
             getattr(L, name).restype = i32
     return L
 

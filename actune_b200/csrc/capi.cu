@@ -10,6 +10,7 @@
 
 #include "actune_b200.h"
 #include "kernels.cuh"
+#include "serving.cuh"
 
 namespace actune {
 namespace {
@@ -498,6 +499,16 @@ int run_rowwise(const uint8_t* a, int A, const float* a_scale, const uint8_t* w,
 }
 
 }  // namespace
+
+int serving_device(int* num_sms) {
+  int dev = 0;
+  const int rc = current_device(&dev);
+  if (rc == ACTUNE_OK) *num_sms = g_devices[dev].num_sms;
+  return rc;
+}
+PFN_cuTensorMapEncodeTiled_v12000 tensor_map_encoder() { return g_encode; }
+int serving_status(cudaError_t e) { return cuda_status(e); }
+
 }  // namespace actune
 
 using namespace actune;

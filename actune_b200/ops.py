@@ -260,3 +260,6 @@ def grouped_linear(x, w, w_scale, bias, W: int, A: int, workspace: torch.Tensor 
             _ptr(workspace), workspace.numel() * workspace.element_size(), int(variant), _stream(dev)),
             "grouped_linear")
     return out
+
+
+from .serving_ops import AdapterPlan, adapter_add, adapter_plan, gated_norm  # noqa: E402,F401

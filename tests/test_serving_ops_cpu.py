@@ -1,0 +1,111 @@
+"""Serving operators without a GPU: the C ABI's symbols and struct layouts, sizes, and
+what the Python calls and the entry points refuse before any device is touched."""
+import ctypes
+import re
+from pathlib import Path
+
+import pytest
+import torch
+
+from actune_b200 import _lib, ops
+
+ROOT = Path(__file__).resolve().parents[1]
+HEADER = (ROOT / "include" / "actune_b200_serving.h").read_text()
+STRUCTS = {"actune_gated_norm_args": _lib.GatedNormArgs, "actune_adapter_args": _lib.AdapterArgs}
+
+
+def test_every_declared_symbol_is_exported_and_bound():
+    declared = set(re.findall(r"^\s*(?:int|size_t)\s+(actune_[a-z0-9_]+)\s*\(", HEADER, flags=re.M))
+    assert declared == set(_lib.SERVING_EXPORTS)
+    library = ctypes.CDLL(str(_lib.LIB_PATH))
+    for name in declared:
+        assert hasattr(library, name)
+
+
+@pytest.mark.parametrize("name", sorted(STRUCTS))
+def test_struct_fields_follow_the_header(name):
+    body = re.search(r"typedef struct %s \{(.*?)\} %s;" % (name, name), HEADER, flags=re.S).group(1)
+    body = re.sub(r"/\*.*?\*/", "", body, flags=re.S)
+    fields = []
+    for line in filter(None, (part.strip() for part in body.split(";"))):
+        kind = ctypes.c_void_p if "*" in line else {"size_t": ctypes.c_size_t, "int64_t": ctypes.c_int64,
+                                                    "int32_t": ctypes.c_int32, "float": ctypes.c_float}[line.split()[0]]
+        names = re.sub(r"^(const )?\w+\s*\**", "", line)
+        fields += [(n.strip(" *"), kind) for n in names.split(",")]
+    assert fields == list(STRUCTS[name]._fields_)
+
+
+def test_entry_points_refuse_before_touching_a_device():
+    L = _lib.lib()
+    for entry, struct in ((L.actune_gated_norm, _lib.GatedNormArgs), (L.actune_adapter_add, _lib.AdapterArgs)):
+        assert entry(None, None) == _lib.ERR_INVALID_VALUE
+        assert entry(ctypes.byref(struct()), None) == _lib.ERR_INVALID_VALUE  # struct_bytes missing
+    size = ctypes.sizeof(_lib.GatedNormArgs)
+    good = dict(struct_bytes=size, T=2, D=64, eps=1e-6, dtype=_lib.DTYPE_BF16, x_stride=64, residual_stride=64)
+    for bad in (dict(T=-1), dict(D=0), dict(dtype=7), dict(quant_bits=3), dict(D=60, quant_bits=8), dict(eps=-1.0),
+                dict(eps=float("nan")), dict(gate_rows=-1), {}):  # the last: null pointers
+        assert L.actune_gated_norm(ctypes.byref(_lib.GatedNormArgs(**{**good, **bad})), None) == _lib.ERR_INVALID_VALUE
+    size = ctypes.sizeof(_lib.AdapterArgs)
+    good = dict(struct_bytes=size, M=4, N=8, K=8, S=2, R=4, x_stride=8, y_stride=8, out_stride=8, tile=16,
+                dtype=_lib.DTYPE_BF16)
+    for bad in (dict(tile=17), dict(R=0), dict(R=129), dict(S=0), dict(S=9000), dict(M=-1), dict(K=0), dict(N=-1),
+                dict(dtype=_lib.DTYPE_F32), dict(out_stride=7)):
+        assert L.actune_adapter_add(ctypes.byref(_lib.AdapterArgs(**{**good, **bad})), None) == _lib.ERR_INVALID_VALUE
+    assert L.actune_adapter_plan(None, 4, 2, 16, None, None) == _lib.ERR_INVALID_VALUE
+
+
+def test_adapter_sizes():
+    L = _lib.lib()
+    # tiles: 100 / 16 full ones and one more for each of 3 adapters and "none"
+    assert L.actune_adapter_plan_size(100, 3, 16) == 4 * (4 + 4 * (6 + 4) + 100)
+    assert L.actune_adapter_plan_size(0, 3, 16) == 16
+    assert L.actune_adapter_plan_size(100, 3, 8) == 0 and L.actune_adapter_plan_size(-1, 3, 16) == 0
+    assert L.actune_adapter_workspace_size(1, 4096, 1, 8, 16) == 32 * 16 * 4  # 32 slices of K, rank padded to 16
+    assert L.actune_adapter_workspace_size(100000, 4096, 1, 100, 64) == 100000 * 128 * 4
+    assert L.actune_adapter_workspace_size(1, 4096, 1, 129, 16) == 0
+
+
+def test_gated_norm_refuses_operands_that_do_not_fit():
+    x, w = torch.zeros(6, 64).bfloat16(), torch.zeros(64).bfloat16()
+
+    def call(match, *args, **kw):
+        with pytest.raises(RuntimeError, match=match):
+            ops.gated_norm(*args, **kw)
+
+    call("CUDA required", x, x, w)
+    call(r"\[T, D\]", x[0], x[0], w)
+    call("one shape", x, x[:4], w)
+    call("one dtype", x, x.half(), w)
+    call("unsupported dtype", x.double(), x.double(), w)
+    call("pre_weight is required", x, x, None)
+    call("last dimension", x.t(), x.t(), w)
+    call("integer width", x, x, w, quant_bits=3)
+    call("multiple of 64", x[:, :60], x[:, :60], w[:60], quant_bits=8)
+
+
+def test_adapter_add_refuses_operands_that_do_not_fit():
+    y, x, s = torch.zeros(6, 32).half(), torch.zeros(6, 16).half(), torch.ones(2)
+    down, up = torch.zeros(2, 4, 16).half(), torch.zeros(2, 32, 4).half()
+    plan = ops.AdapterPlan(torch.zeros(64, dtype=torch.int32), 6, 2, 16)
+
+    def call(match, *args, **kw):
+        with pytest.raises(RuntimeError, match=match):
+            ops.adapter_add(*args, **kw)
+
+    call("CUDA required", y, x, down, up, s, plan)
+    call("x and y must be", y[0], x[0], down, up, s, plan)
+    call("x and y must be", y, x[:5], down, up, s, plan)
+    call("down must be", y, x, down[:, :, :8], up, s, plan)
+    call("down must be", y, x, down, up[:, :, :2], s, plan)
+    call("rank", y, x, torch.zeros(2, 129, 16).half(), torch.zeros(2, 32, 129).half(), s, plan)
+    call("unsupported dtype", y.float(), x.float(), down, up, s, plan)
+    call("one dtype", y, x.bfloat16(), down, up, s, plan)
+    call("scale", y, x, down, up, s.half(), plan)
+    call("contiguous adapters", y, x, torch.zeros(2, 16, 4).half().transpose(1, 2), up, s, plan)
+    call("the plan is for", y[:5], x[:5], down, up, s, plan)
+    call("out must match", y, x, down, up, s, plan, out=y[:5])
+    call("must not overlap", y, x, down, up, s, plan, out=y[:1].expand(6, 32))
+    with pytest.raises(RuntimeError, match="int32"):
+        ops.adapter_plan(torch.zeros(4, dtype=torch.int64), 2)
+    with pytest.raises(RuntimeError, match="CUDA required"):
+        ops.adapter_plan(torch.zeros(4, dtype=torch.int32), 2)
