@@ -59,6 +59,8 @@ SERVING_EXPORTS = (
     "actune_adapter_plan",
     "actune_adapter_workspace_size",
     "actune_adapter_add",
+    "actune_prefix_attention_workspace_size",
+    "actune_prefix_attention",
 )
 
 _LIB = None
@@ -85,6 +87,20 @@ class AdapterArgs(ctypes.Structure):
                 + [("workspace_bytes", ctypes.c_size_t)]
                 + [(n, ctypes.c_int64) for n in ("M", "N", "K", "S", "R", "x_stride", "y_stride", "out_stride")]
                 + [(n, ctypes.c_int32) for n in ("tile", "dtype")])
+
+
+class PrefixAttentionArgs(ctypes.Structure):
+    """actune_prefix_attention_args (include/actune_b200_serving.h)."""
+
+    _fields_ = ([("struct_bytes", ctypes.c_size_t)]
+                + [(n, ctypes.c_void_p) for n in ("q", "prefix_k", "prefix_v", "k", "v", "starts", "prefix_lens", "lens",
+                                                  "out", "workspace")]
+                + [("workspace_bytes", ctypes.c_size_t)]
+                + [(n, ctypes.c_int64) for n in ("B", "T", "H", "KV", "D", "G", "P", "S", "q_b", "q_t", "q_h", "pk_g",
+                                                 "pk_p", "pk_h", "pv_g", "pv_p", "pv_h", "k_b", "k_s", "k_h", "v_b",
+                                                 "v_s", "v_h")]
+                + [("scale", ctypes.c_float)]
+                + [(n, ctypes.c_int32) for n in ("dtype", "causal")])
 
 
 class ActuneError(RuntimeError):
@@ -125,6 +141,8 @@ def _declare(L):
     L.actune_adapter_plan.argtypes = [p, i64, i64, i32, p, p]
     L.actune_adapter_workspace_size.argtypes = [i64, i64, i64, i64, i32]
     L.actune_adapter_add.argtypes = [ctypes.POINTER(AdapterArgs), p]
+    L.actune_prefix_attention_workspace_size.argtypes = [i64] * 8
+    L.actune_prefix_attention.argtypes = [ctypes.POINTER(PrefixAttentionArgs), p]
     for name in EXPORTS + SERVING_EXPORTS:
         if name.endswith("_size"):
             getattr(L, name).restype = sz

@@ -262,4 +262,5 @@ def grouped_linear(x, w, w_scale, bias, W: int, A: int, workspace: torch.Tensor 
     return out
 
 
-from .serving_ops import AdapterPlan, adapter_add, adapter_plan, gated_norm  # noqa: E402,F401
+from .serving_ops import (AdapterPlan, adapter_add, adapter_plan, gated_norm,  # noqa: E402,F401
+                          shared_prefix_attention)

@@ -1,6 +1,7 @@
 """Tensor-level calls of the serving operators (include/actune_b200_serving.h),
 re-exported by ``actune_b200.ops``.
 
+* ``shared_prefix_attention``: attention of a batch whose sequences share prefixes.
 * ``adapter_plan`` / ``adapter_add``: low-rank adapters of many requests added to the
   output of the projection they share.
 * ``gated_norm``: norm after a block, gate, residual scale and the norm before the
@@ -202,4 +203,70 @@ def adapter_add(y, x, down, up, scale, plan, *, out=None):
         _ptr(out), _ptr(workspace), size, rows, n, k, slots, rank, _row_stride(x), _row_stride(y), _row_stride(out),
         plan.tile, _DTYPES[x.dtype])
     _call(L.actune_adapter_add, "adapter_add", device, args)
+    return out
+
+
+# ------------------------------------------------------------------------- attention
+def _lengths(t, count, device, name):
+    if t is not None:
+        _require(t.dtype == torch.int32 and t.dim() == 1 and t.shape[0] == count and t.is_contiguous(),
+                 f"{name} must be a contiguous int32 vector of {count}")
+        _require(t.device == device, f"device mismatch: {name}")
+
+
+def shared_prefix_attention(q, prefix_k, prefix_v, k, v, *, starts=None, prefix_lens=None, lens=None, causal=False,
+                            scale=None, out=None):
+    """Attention of a batch whose sequences share prefixes, each prefix's keys and values
+    held (and, for few query rows, read) once for all the sequences behind it.
+
+    q [B, T, H, D]: T query tokens of each of B sequences; prefix_k / prefix_v
+    [G, P, KV, D]: G prefixes; k / v [B, S, KV, D]: the sequences' own keys and values
+    (S may be 0).  Query head h reads key/value head h // (H // KV).  Sequences
+    starts[g] .. starts[g + 1] - 1 share prefix g (int32 [G + 1], non-decreasing from 0
+    to B; by default the B sequences are dealt evenly, sequence b to prefix b * G // B).
+    The first prefix_lens[g] rows of a prefix and the first lens[b] of a sequence's own
+    count (int32; all by default); what lies behind them is never used, whatever it
+    holds.  Every query sees its whole prefix; with ``causal`` query t sees own key j for
+    j <= lens[b] - T + t, without it all of them.  A query that sees nothing gets zeros.
+    ``scale`` (positive) defaults to D ** -0.5.
+
+    float16 or bfloat16, D <= 256 contiguous, any other strides: cache views such as
+    cache[:, :, 0].unsqueeze(2) and slices of a fused projection need no copy.  With D a
+    multiple of 8 and 16-byte aligned rows it runs on the tensor cores, otherwise on a
+    scalar kernel many times slower.  Returns [B, T, H, D], contiguous."""
+    for t in (q, prefix_k, prefix_v, k, v):
+        _require(t.dim() == 4, "q, prefix_k, prefix_v, k and v must be 4-D")
+    B, T, H, D = q.shape
+    G, P, KV, _ = prefix_k.shape
+    S = k.shape[1]
+    code = _DTYPES.get(q.dtype)
+    _require(code in (_lib.DTYPE_F16, _lib.DTYPE_BF16), f"unsupported dtype {q.dtype} (float16 or bfloat16 required)")
+    _require(G > 0 and KV > 0 and H % KV == 0, "the query heads must be a multiple of the key/value heads")
+    _require(1 <= D <= 256, "the head size must be between 1 and 256")
+    _require(tuple(prefix_k.shape) == (G, P, KV, D) and prefix_v.shape == prefix_k.shape,
+             f"prefix_k and prefix_v must be [G, P, KV, {D}]")
+    _require(tuple(k.shape) == (B, S, KV, D) and v.shape == k.shape, f"k and v must be [{B}, S, {KV}, {D}]")
+    for t in (prefix_k, prefix_v, k, v):
+        _require(t.dtype == q.dtype, "q, keys and values must have one dtype")
+    for t in (q, prefix_k, prefix_v, k, v):
+        _require(D == 1 or t.stride(3) == 1, "the last dimension must be contiguous")
+    device = _same_device(q, prefix_k=prefix_k, prefix_v=prefix_v, k=k, v=v, out=out)
+    _lengths(starts, G + 1, device, "starts")
+    _lengths(prefix_lens, G, device, "prefix_lens")
+    _lengths(lens, B, device, "lens")
+    scale = D ** -0.5 if scale is None else float(scale)
+    _require(0.0 < scale < 3e38, "scale must be positive and finite")
+    if out is None:
+        out = torch.empty((B, T, H, D), device=device, dtype=q.dtype)
+    _require(out.shape == q.shape and out.dtype == q.dtype and out.is_contiguous(),
+             "out must be contiguous and match q")
+    L = _lib.lib()
+    size = L.actune_prefix_attention_workspace_size(B, T, H, KV, D, G, P, S)
+    workspace = torch.empty(size, device=device, dtype=torch.uint8) if size else None
+    args = _lib.PrefixAttentionArgs(
+        ctypes.sizeof(_lib.PrefixAttentionArgs), _ptr(q), _ptr(prefix_k), _ptr(prefix_v), _ptr(k), _ptr(v),
+        _ptr(starts), _ptr(prefix_lens), _ptr(lens), _ptr(out), _ptr(workspace), size, B, T, H, KV, D, G, P, S,
+        *q.stride()[:3], *prefix_k.stride()[:3], *prefix_v.stride()[:3], *k.stride()[:3], *v.stride()[:3], scale, code,
+        bool(causal))
+    _call(L.actune_prefix_attention, "shared_prefix_attention", device, args)
     return out

@@ -92,6 +92,51 @@ typedef struct actune_adapter_args {
 size_t actune_adapter_workspace_size(int64_t M, int64_t K, int64_t S, int64_t R, int tile);
 int actune_adapter_add(const actune_adapter_args* args, void* stream);
 
+/* Attention of a batch whose sequences share long prefixes.  Sequence b has T query
+ * tokens, S rows of keys and values of its own, of which the first lens[b] count, and
+ * the prefix g it belongs to (starts[g] <= b < starts[g + 1]), of P rows, of which the
+ * first prefix_lens[g] count.  Query head h reads key/value head h / (H / KV).
+ *     out[b, t, h] = sum_j p_j v_j,  p = softmax over the keys seen of scale * q . k_j
+ * over the prefix and the sequence's own keys; with causal != 0, query t sees own key j
+ * only for j <= lens[b] - T + t.  A query that sees no key gets zeros, and rows of the
+ * caches that nothing sees are not used whatever they hold.
+ * starts: int32 [G + 1], non-decreasing from 0 to B (NULL: sequence b has prefix
+ * b * G / B); prefix_lens, lens: int32 [G], [B] (NULL: all of P, S; values outside are
+ * clamped).  All three are read on the device.
+ * q [B, T, H, D], prefix_k and prefix_v [G, P, KV, D], k and v [B, S, KV, D], D <= 256,
+ * of `dtype` (F16 or BF16), with D contiguous and the given strides; out [B, T, H, D]
+ * contiguous.  Scores, softmax and sums are fp32; p is rounded to `dtype` for the
+ * product with V, as the tensor core takes it.
+ * workspace: at least actune_prefix_attention_workspace_size bytes, 16-byte aligned.
+ * Operands with D a multiple of 8, 16-byte aligned, and strides that are positive
+ * multiples of 8 run on the tensor cores; others on a scalar kernel. */
+typedef struct actune_prefix_attention_args {
+  size_t struct_bytes;
+  const void* q;
+  const void* prefix_k;
+  const void* prefix_v;
+  const void* k;
+  const void* v;
+  const int32_t* starts;
+  const int32_t* prefix_lens;
+  const int32_t* lens;
+  void* out;
+  void* workspace;
+  size_t workspace_bytes;
+  int64_t B, T, H, KV, D, G, P, S;
+  int64_t q_b, q_t, q_h;    /* strides of q by sequence, token and head */
+  int64_t pk_g, pk_p, pk_h; /* of prefix_k by prefix, row and head */
+  int64_t pv_g, pv_p, pv_h;
+  int64_t k_b, k_s, k_h;
+  int64_t v_b, v_s, v_h;
+  float scale;
+  int32_t dtype, causal;
+} actune_prefix_attention_args;
+
+size_t actune_prefix_attention_workspace_size(int64_t B, int64_t T, int64_t H, int64_t KV, int64_t D, int64_t G,
+                                              int64_t P, int64_t S);
+int actune_prefix_attention(const actune_prefix_attention_args* args, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

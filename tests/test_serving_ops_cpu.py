@@ -11,7 +11,8 @@ from actune_b200 import _lib, ops
 
 ROOT = Path(__file__).resolve().parents[1]
 HEADER = (ROOT / "include" / "actune_b200_serving.h").read_text()
-STRUCTS = {"actune_gated_norm_args": _lib.GatedNormArgs, "actune_adapter_args": _lib.AdapterArgs}
+STRUCTS = {"actune_gated_norm_args": _lib.GatedNormArgs, "actune_adapter_args": _lib.AdapterArgs,
+           "actune_prefix_attention_args": _lib.PrefixAttentionArgs}
 
 
 def test_every_declared_symbol_is_exported_and_bound():
@@ -37,7 +38,8 @@ def test_struct_fields_follow_the_header(name):
 
 def test_entry_points_refuse_before_touching_a_device():
     L = _lib.lib()
-    for entry, struct in ((L.actune_gated_norm, _lib.GatedNormArgs), (L.actune_adapter_add, _lib.AdapterArgs)):
+    for entry, struct in ((L.actune_gated_norm, _lib.GatedNormArgs), (L.actune_adapter_add, _lib.AdapterArgs),
+                          (L.actune_prefix_attention, _lib.PrefixAttentionArgs)):
         assert entry(None, None) == _lib.ERR_INVALID_VALUE
         assert entry(ctypes.byref(struct()), None) == _lib.ERR_INVALID_VALUE  # struct_bytes missing
     size = ctypes.sizeof(_lib.GatedNormArgs)
@@ -52,6 +54,37 @@ def test_entry_points_refuse_before_touching_a_device():
                 dict(dtype=_lib.DTYPE_F32), dict(out_stride=7)):
         assert L.actune_adapter_add(ctypes.byref(_lib.AdapterArgs(**{**good, **bad})), None) == _lib.ERR_INVALID_VALUE
     assert L.actune_adapter_plan(None, 4, 2, 16, None, None) == _lib.ERR_INVALID_VALUE
+
+
+def test_attention_entry_refuses_before_touching_a_device():
+    L = _lib.lib()
+    good = dict(struct_bytes=ctypes.sizeof(_lib.PrefixAttentionArgs), B=2, T=1, H=4, KV=2, D=64, G=1, P=8, S=4,
+                scale=0.125, dtype=_lib.DTYPE_BF16)
+    for bad in (dict(H=3), dict(KV=0), dict(D=0), dict(D=257), dict(G=0), dict(P=-1), dict(S=-1), dict(scale=0.0),
+                dict(scale=-1.0), dict(scale=float("nan")), dict(scale=float("inf")), dict(dtype=_lib.DTYPE_F32),
+                dict(pk_p=-64), dict(B=1 << 21), dict(T=1 << 25)):
+        args = _lib.PrefixAttentionArgs(**{**good, **bad})
+        assert L.actune_prefix_attention(ctypes.byref(args), None) == _lib.ERR_INVALID_VALUE, bad
+
+
+def test_attention_refuses_operands_that_do_not_fit():
+    q, pk, k = torch.zeros(4, 2, 4, 64).half(), torch.zeros(2, 9, 2, 64).half(), torch.zeros(4, 5, 2, 64).half()
+
+    def call(match, *args, **kw):
+        with pytest.raises(RuntimeError, match=match):
+            ops.shared_prefix_attention(*args, **kw)
+
+    call("CUDA required", q, pk, pk, k, k)
+    call("4-D", q[0], pk, pk, k, k)
+    call("unsupported dtype", q.float(), pk, pk, k, k)
+    call("multiple of the key/value heads", q[:, :, :3], pk, pk, k, k)
+    call("head size", torch.zeros(4, 2, 4, 264).half(), torch.zeros(2, 9, 2, 264).half(), pk, k, k)
+    call("prefix_k and prefix_v", q, pk, pk[:, :8], k, k)
+    call("prefix_k and prefix_v", q, pk[..., :32], pk[..., :32], k, k)
+    call("k and v must be", q, pk, pk, k[:3], k[:3])
+    call("k and v must be", q, pk, pk, k[:, :, :1], k[:, :, :1])
+    call("one dtype", q, pk.bfloat16(), pk, k, k)
+    call("last dimension", q, pk.transpose(1, 3).contiguous().transpose(1, 3), pk, k, k)
 
 
 def test_adapter_sizes():
