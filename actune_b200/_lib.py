@@ -67,42 +67,6 @@ _LIB = None
 _LOCK = threading.Lock()
 
 
-class GatedNormArgs(ctypes.Structure):
-    """actune_gated_norm_args (include/actune_b200_serving.h)."""
-
-    _fields_ = ([("struct_bytes", ctypes.c_size_t)]
-                + [(n, ctypes.c_void_p) for n in ("x", "residual", "post_weight", "pre_weight", "gate", "shift", "out",
-                                                  "residual_out", "packed", "scales")]
-                + [(n, ctypes.c_int64) for n in ("T", "D", "x_stride", "residual_stride", "post_rows", "pre_rows",
-                                                 "gate_rows", "shift_rows")]
-                + [("residual_scale", ctypes.c_float), ("eps", ctypes.c_float)]
-                + [(n, ctypes.c_int32) for n in ("dtype", "gemma", "quant_bits", "codes8")])
-
-
-class AdapterArgs(ctypes.Structure):
-    """actune_adapter_args (include/actune_b200_serving.h)."""
-
-    _fields_ = ([("struct_bytes", ctypes.c_size_t)]
-                + [(n, ctypes.c_void_p) for n in ("x", "y", "down", "up", "scale", "plan", "out", "workspace")]
-                + [("workspace_bytes", ctypes.c_size_t)]
-                + [(n, ctypes.c_int64) for n in ("M", "N", "K", "S", "R", "x_stride", "y_stride", "out_stride")]
-                + [(n, ctypes.c_int32) for n in ("tile", "dtype")])
-
-
-class PrefixAttentionArgs(ctypes.Structure):
-    """actune_prefix_attention_args (include/actune_b200_serving.h)."""
-
-    _fields_ = ([("struct_bytes", ctypes.c_size_t)]
-                + [(n, ctypes.c_void_p) for n in ("q", "prefix_k", "prefix_v", "k", "v", "starts", "prefix_lens", "lens",
-                                                  "out", "workspace")]
-                + [("workspace_bytes", ctypes.c_size_t)]
-                + [(n, ctypes.c_int64) for n in ("B", "T", "H", "KV", "D", "G", "P", "S", "q_b", "q_t", "q_h", "pk_g",
-                                                 "pk_p", "pk_h", "pv_g", "pv_p", "pv_h", "k_b", "k_s", "k_h", "v_b",
-                                                 "v_s", "v_h")]
-                + [("scale", ctypes.c_float)]
-                + [(n, ctypes.c_int32) for n in ("dtype", "causal")])
-
-
 class ActuneError(RuntimeError):
     """A C-ABI call returned a non-zero actune_status."""
 
@@ -136,13 +100,13 @@ def _declare(L):
     L.actune_set_wait_limit_ns.argtypes = [ctypes.c_uint64]
     L.actune_wait_limit_ns.argtypes = [ctypes.POINTER(ctypes.c_uint64)]
     L.actune_selftest_wait_timeout.argtypes = [i32, p]
-    L.actune_gated_norm.argtypes = [ctypes.POINTER(GatedNormArgs), p]
+    L.actune_gated_norm.argtypes = [p, p]
     L.actune_adapter_plan_size.argtypes = [i64, i64, i32]
     L.actune_adapter_plan.argtypes = [p, i64, i64, i32, p, p]
     L.actune_adapter_workspace_size.argtypes = [i64, i64, i64, i64, i32]
-    L.actune_adapter_add.argtypes = [ctypes.POINTER(AdapterArgs), p]
+    L.actune_adapter_add.argtypes = [p, p]
     L.actune_prefix_attention_workspace_size.argtypes = [i64] * 8
-    L.actune_prefix_attention.argtypes = [ctypes.POINTER(PrefixAttentionArgs), p]
+    L.actune_prefix_attention.argtypes = [p, p]
     for name in EXPORTS + SERVING_EXPORTS:
         if name.endswith("_size"):
             getattr(L, name).restype = sz

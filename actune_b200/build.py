@@ -6,6 +6,9 @@ Each csrc/*.cu is compiled to an object with relocatable device code (the
 device error word is shared by all kernels), then nvcc device-links them into
 one shared library next to this file.  The CUDA runtime is linked statically so
 the library only needs the driver at run time.
+
+csrc/torch/*.cpp is host code against torch's headers: g++ compiles it into the CPython
+module _serving.so, which links the library above (found next to it).
 """
 from __future__ import annotations
 
@@ -14,6 +17,7 @@ import concurrent.futures as cf
 import os
 import shutil
 import subprocess
+import sysconfig
 from pathlib import Path
 
 PKG = Path(__file__).resolve().parent
@@ -21,6 +25,8 @@ CSRC = PKG / "csrc"
 INCLUDE = PKG.parent / "include"
 BUILD = PKG / "_build"
 LIB = PKG / "libactune_b200.so"
+TORCH_SOURCE = CSRC / "torch" / "serving.cpp"
+TORCH_MODULE = PKG / "_serving.so"
 
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
 NVCC_FLAGS = ["-O3", "-lineinfo", "-std=c++17", "-rdc=true", "-Xcompiler", "-fPIC,-O2",
@@ -77,7 +83,29 @@ def build(force: bool = False, verbose_ptxas: bool = False, jobs: int | None = N
         r = subprocess.run(cmd, capture_output=True, text=True)
         if r.returncode != 0:
             raise RuntimeError(f"nvcc link failed:\n{r.stdout}\n{r.stderr}")
+    if out is None:
+        build_torch_module(force)
     return lib
+
+
+def build_torch_module(force: bool = False) -> Path:
+    """Compile the CPython module of the serving operators (needs torch's headers and the
+    built library)."""
+    if not force and not _stale(TORCH_MODULE, [TORCH_SOURCE, Path(__file__), *INCLUDE.glob("*.h")]):
+        return TORCH_MODULE
+    import torch
+    from torch.utils import cpp_extension
+    cuda = Path(nvcc()).resolve().parents[1]
+    includes = [INCLUDE, *cpp_extension.include_paths(), cuda / "include", sysconfig.get_paths()["include"]]
+    cmd = [os.environ.get("CXX", "g++"), "-O2", "-std=c++20", "-shared", "-fPIC", "-fvisibility=hidden",
+           f"-D_GLIBCXX_USE_CXX11_ABI={int(torch.compiled_with_cxx11_abi())}",
+           *(f"-isystem{d}" for d in includes), str(TORCH_SOURCE), "-o", str(TORCH_MODULE),
+           f"-L{PKG}", "-lactune_b200", "-Wl,-rpath,$ORIGIN",
+           f"-L{Path(torch.__file__).parent / 'lib'}", "-ltorch_python", "-ltorch_cpu", "-ltorch", "-lc10_cuda", "-lc10"]
+    r = subprocess.run(cmd, capture_output=True, text=True)
+    if r.returncode != 0:
+        raise RuntimeError(f"g++ failed for {TORCH_SOURCE.name}:\n{r.stdout}\n{r.stderr}")
+    return TORCH_MODULE
 
 
 def main():

@@ -11,8 +11,21 @@ from actune_b200 import _lib, ops
 
 ROOT = Path(__file__).resolve().parents[1]
 HEADER = (ROOT / "include" / "actune_b200_serving.h").read_text()
-STRUCTS = {"actune_gated_norm_args": _lib.GatedNormArgs, "actune_adapter_args": _lib.AdapterArgs,
-           "actune_prefix_attention_args": _lib.PrefixAttentionArgs}
+
+
+def struct_of(name):
+    """The header's struct as a ctypes class."""
+    body = re.search(r"typedef struct %s \{(.*?)\} %s;" % (name, name), HEADER, flags=re.S).group(1)
+    fields = []
+    for line in filter(None, (part.strip() for part in re.sub(r"/\*.*?\*/", "", body, flags=re.S).split(";"))):
+        kind = ctypes.c_void_p if "*" in line else {"size_t": ctypes.c_size_t, "int64_t": ctypes.c_int64,
+                                                    "int32_t": ctypes.c_int32, "float": ctypes.c_float}[line.split()[0]]
+        fields += [(n.strip(" *"), kind) for n in re.sub(r"^(const )?\w+\s*\**", "", line).split(",")]
+    return type(name, (ctypes.Structure,), {"_fields_": fields})
+
+
+GatedNormArgs, AdapterArgs, PrefixAttentionArgs = (struct_of(f"actune_{n}_args") for n in (
+    "gated_norm", "adapter", "prefix_attention"))
 
 
 def test_every_declared_symbol_is_exported_and_bound():
@@ -23,47 +36,34 @@ def test_every_declared_symbol_is_exported_and_bound():
         assert hasattr(library, name)
 
 
-@pytest.mark.parametrize("name", sorted(STRUCTS))
-def test_struct_fields_follow_the_header(name):
-    body = re.search(r"typedef struct %s \{(.*?)\} %s;" % (name, name), HEADER, flags=re.S).group(1)
-    body = re.sub(r"/\*.*?\*/", "", body, flags=re.S)
-    fields = []
-    for line in filter(None, (part.strip() for part in body.split(";"))):
-        kind = ctypes.c_void_p if "*" in line else {"size_t": ctypes.c_size_t, "int64_t": ctypes.c_int64,
-                                                    "int32_t": ctypes.c_int32, "float": ctypes.c_float}[line.split()[0]]
-        names = re.sub(r"^(const )?\w+\s*\**", "", line)
-        fields += [(n.strip(" *"), kind) for n in names.split(",")]
-    assert fields == list(STRUCTS[name]._fields_)
-
-
 def test_entry_points_refuse_before_touching_a_device():
     L = _lib.lib()
-    for entry, struct in ((L.actune_gated_norm, _lib.GatedNormArgs), (L.actune_adapter_add, _lib.AdapterArgs),
-                          (L.actune_prefix_attention, _lib.PrefixAttentionArgs)):
+    for entry, struct in ((L.actune_gated_norm, GatedNormArgs), (L.actune_adapter_add, AdapterArgs),
+                          (L.actune_prefix_attention, PrefixAttentionArgs)):
         assert entry(None, None) == _lib.ERR_INVALID_VALUE
         assert entry(ctypes.byref(struct()), None) == _lib.ERR_INVALID_VALUE  # struct_bytes missing
-    size = ctypes.sizeof(_lib.GatedNormArgs)
+    size = ctypes.sizeof(GatedNormArgs)
     good = dict(struct_bytes=size, T=2, D=64, eps=1e-6, dtype=_lib.DTYPE_BF16, x_stride=64, residual_stride=64)
     for bad in (dict(T=-1), dict(D=0), dict(dtype=7), dict(quant_bits=3), dict(D=60, quant_bits=8), dict(eps=-1.0),
                 dict(eps=float("nan")), dict(gate_rows=-1), {}):  # the last: null pointers
-        assert L.actune_gated_norm(ctypes.byref(_lib.GatedNormArgs(**{**good, **bad})), None) == _lib.ERR_INVALID_VALUE
-    size = ctypes.sizeof(_lib.AdapterArgs)
+        assert L.actune_gated_norm(ctypes.byref(GatedNormArgs(**{**good, **bad})), None) == _lib.ERR_INVALID_VALUE
+    size = ctypes.sizeof(AdapterArgs)
     good = dict(struct_bytes=size, M=4, N=8, K=8, S=2, R=4, x_stride=8, y_stride=8, out_stride=8, tile=16,
                 dtype=_lib.DTYPE_BF16)
     for bad in (dict(tile=17), dict(R=0), dict(R=129), dict(S=0), dict(S=9000), dict(M=-1), dict(K=0), dict(N=-1),
                 dict(dtype=_lib.DTYPE_F32), dict(out_stride=7)):
-        assert L.actune_adapter_add(ctypes.byref(_lib.AdapterArgs(**{**good, **bad})), None) == _lib.ERR_INVALID_VALUE
+        assert L.actune_adapter_add(ctypes.byref(AdapterArgs(**{**good, **bad})), None) == _lib.ERR_INVALID_VALUE
     assert L.actune_adapter_plan(None, 4, 2, 16, None, None) == _lib.ERR_INVALID_VALUE
 
 
 def test_attention_entry_refuses_before_touching_a_device():
     L = _lib.lib()
-    good = dict(struct_bytes=ctypes.sizeof(_lib.PrefixAttentionArgs), B=2, T=1, H=4, KV=2, D=64, G=1, P=8, S=4,
+    good = dict(struct_bytes=ctypes.sizeof(PrefixAttentionArgs), B=2, T=1, H=4, KV=2, D=64, G=1, P=8, S=4,
                 scale=0.125, dtype=_lib.DTYPE_BF16)
     for bad in (dict(H=3), dict(KV=0), dict(D=0), dict(D=257), dict(G=0), dict(P=-1), dict(S=-1), dict(scale=0.0),
                 dict(scale=-1.0), dict(scale=float("nan")), dict(scale=float("inf")), dict(dtype=_lib.DTYPE_F32),
                 dict(pk_p=-64), dict(B=1 << 21), dict(T=1 << 25)):
-        args = _lib.PrefixAttentionArgs(**{**good, **bad})
+        args = PrefixAttentionArgs(**{**good, **bad})
         assert L.actune_prefix_attention(ctypes.byref(args), None) == _lib.ERR_INVALID_VALUE, bad
 
 
