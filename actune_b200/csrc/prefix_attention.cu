@@ -37,6 +37,24 @@ constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kRescale = 8.f;  // growth of the maximum (log2) that O is rescaled for
 constexpr int kSiteAttn = 300;
 
+// n / d for 0 <= n < 2^31 by multiplication: an item's place in the grid and a row's
+// place in its sequence are several divisions deep before the first load can start.
+struct Divisor {
+  uint32_t d, mul, shift;
+  void set(int64_t by) {
+    d = (uint32_t)by, shift = 0;
+    while (((uint64_t)1 << shift) < d) ++shift;
+    mul = (uint32_t)((((uint64_t)1 << 32) * (((uint64_t)1 << shift) - d)) / d + 1);
+  }
+  __device__ __forceinline__ int div(int n) const { return (int)((__umulhi((uint32_t)n, mul) + (uint32_t)n) >> shift); }
+  // n -> n / d, the remainder returned.
+  __device__ __forceinline__ int split(int& n) const {
+    const int q = div(n), r = n - q * (int)d;
+    n = q;
+    return r;
+  }
+};
+
 struct AttnParams {
   const void *q, *pk, *pv, *k, *v;
   const int32_t *starts, *prefix_lens, *lens;
@@ -53,6 +71,8 @@ struct AttnParams {
   int prefix_tiles; // upper bound on the stacked tiles of a key/value head
   int prefix_splits, own_splits;  // by sequence: prefix_splits of both together
   int splits;       // parts per row; 1: write out directly
+  int q_boxes;      // query tiles come by tensor map (tokens evenly spaced, rep a divisor of 128)
+  Divisor by_prefix_tiles, by_kv, by_own_tiles, by_tiles_per_seq, by_per_seq, by_rep, by_prefix_splits, by_own_splits;
 };
 
 __device__ __forceinline__ int clamp_len(const int32_t* lens, int i, int most) {
@@ -176,6 +196,14 @@ __device__ __forceinline__ void tmem_st32(uint32_t taddr, const uint32_t* r) {
       : "memory");
 }
 
+__device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t* r) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};" ::"r"(taddr),
+      "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]),
+      "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
+      : "memory");
+}
+
 __device__ __forceinline__ void tma_load_4d(uint32_t dst, const CUtensorMap* map, int x, int y, int z, int w,
                                             uint32_t bar) {
   asm volatile(
@@ -184,6 +212,37 @@ __device__ __forceinline__ void tma_load_4d(uint32_t dst, const CUtensorMap* map
       "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(z), "r"(w), "r"(bar)
       : "memory");
 }
+
+// Waits for this thread's loads from tensor memory; the operands keep the uses of what was
+// loaded behind the wait.
+__device__ __forceinline__ void tmem_wait_ld32(uint32_t (&r)[32]) {
+  asm volatile("tcgen05.wait::ld.sync.aligned;"
+               : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]),
+                 "+r"(r[8]), "+r"(r[9]), "+r"(r[10]), "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15])
+               :
+               : "memory");
+  asm volatile(""
+               : "+r"(r[16]), "+r"(r[17]), "+r"(r[18]), "+r"(r[19]), "+r"(r[20]), "+r"(r[21]), "+r"(r[22]),
+                 "+r"(r[23]), "+r"(r[24]), "+r"(r[25]), "+r"(r[26]), "+r"(r[27]), "+r"(r[28]), "+r"(r[29]),
+                 "+r"(r[30]), "+r"(r[31])
+               :
+               : "memory");
+}
+
+__device__ __forceinline__ void tmem_wait_ld16(uint32_t (&r)[16]) {
+  asm volatile("tcgen05.wait::ld.sync.aligned;"
+               : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]),
+                 "+r"(r[8]), "+r"(r[9]), "+r"(r[10]), "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15])
+               :
+               : "memory");
+}
+
+// 16 bytes global -> shared without a register in between (all of a thread's are in
+// flight at once); zeros when !there.
+__device__ __forceinline__ void copy16_or_zero(uint32_t dst, const void* src, bool there) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(there ? 16 : 0) : "memory");
+}
+__device__ __forceinline__ void copy16_wait() { asm volatile("cp.async.wait_all;" ::: "memory"); }
 
 __device__ __forceinline__ float exp2_approx(float x) {
   float y;
@@ -208,16 +267,18 @@ __device__ __forceinline__ uint32_t pack16<__half>(float a, float b) {
 // NT: row tiles of 128 per CTA.
 template <int DP, int NT>
 struct AttnCfg {
-  static constexpr int BN = DP > 128 ? 64 : 128;       // keys per block
+  static constexpr int BN = 64;  // keys per block
+  static constexpr int NB = 2;   // score buffers per tile: the next block's are computed ahead
   static constexpr int ROWS = 128 * NT;
   static constexpr int Q_BYTES = ROWS * DP * 2;
   static constexpr int SLOT_BYTES = BN * DP * 2;        // one K or V block
-  static constexpr int RING = (224 * 1024 - Q_BYTES) / SLOT_BYTES > 8 ? 8 : (224 * 1024 - Q_BYTES) / SLOT_BYTES;
+  static constexpr int FIT = (226 * 1024 - 512 - NT * 1024 - Q_BYTES) / SLOT_BYTES;  // beside the static arrays
+  static constexpr int RING = FIT > 12 ? 12 : FIT;
   static constexpr int SMEM = 1024 + Q_BYTES + RING * SLOT_BYTES;
-  static constexpr int O_COL = 0, S_COL = NT * DP;      // tensor memory columns: O, then two score buffers
+  static constexpr int O_COL = 0, S_COL = NT * DP;      // tensor memory columns: O, then the score buffers
   static constexpr int TMEM_COLS = 512;
-  static constexpr int WARPS = 4 * NT + 2;
-  static_assert(S_COL + 2 * BN <= TMEM_COLS && RING >= 4 && SMEM + 512 <= 227 * 1024, "fits");
+  static constexpr int WARPS = 8 * NT + 1 + NT;         // softmax, producer, issuers
+  static_assert(S_COL + NT * NB * BN <= TMEM_COLS && RING >= NB + 2 && SMEM + NT * 1024 + 512 <= 227 * 1024, "fits");
 };
 
 struct AttnItem {
@@ -236,10 +297,16 @@ __device__ AttnItem attn_item(const AttnParams& p, int lane) {
   const int per_seq = p.T * p.rep;
   int x = blockIdx.x;
   const int prefix_items = p.stacked ? p.prefix_tiles * p.KV * p.prefix_splits : 0;
+  // Part `i` of `blocks` blocks dealt to d.d parts: [begin, end).
+  const auto deal = [](int blocks, const Divisor& d, int i, int& begin, int& end) {
+    int each = blocks;
+    const int more = d.split(each);  // that many parts get one more
+    begin = i * each + min(i, more);
+    end = begin + each + (i < more);
+  };
   if (x < prefix_items) {
-    const int tile = x % p.prefix_tiles;
-    x /= p.prefix_tiles;
-    it.kv = x % p.KV, it.split = x / p.KV;
+    const int tile = p.by_prefix_tiles.split(x);
+    it.kv = p.by_kv.split(x), it.split = x;
     // The prefix whose stacked rows hold this tile: running count of tiles, 32 prefixes a step.
     int before = 0;
     bool found = false;
@@ -277,28 +344,23 @@ __device__ AttnItem attn_item(const AttnParams& p, int lane) {
     if (!found) return it;
     it.b = it.seq0;
     it.plen = clamp_len(p.prefix_lens, it.g, p.P);
-    const int64_t blocks = (it.plen + BN - 1) / BN;
-    it.pb0 = (int)(blocks * it.split / p.prefix_splits);
-    it.pb1 = (int)(blocks * (it.split + 1) / p.prefix_splits);
+    deal((it.plen + BN - 1) / BN, p.by_prefix_splits, it.split, it.pb0, it.pb1);
     return it;
   }
   x -= prefix_items;
-  const int tiles = p.B * p.tiles_per_seq;
-  const int tile = x % tiles;
-  x /= tiles;
-  it.kv = x % p.KV;
-  const int part = x / p.KV;
-  it.b = it.seq0 = tile / p.tiles_per_seq;
-  it.row0 = tile % p.tiles_per_seq * ROWS;
+  int tile = p.by_own_tiles.split(x);
+  it.kv = p.by_kv.split(x);
+  const int part = x;
+  it.row0 = p.by_tiles_per_seq.split(tile) * ROWS;
+  it.b = it.seq0 = tile;
   it.nrows = min(ROWS, per_seq - it.row0);
   it.slen = clamp_len(p.lens, it.b, p.S);
   int seen = it.slen;  // own keys that the tile's last row sees
-  if (p.causal) seen = max(0, min(seen, it.slen - p.T + (it.row0 + it.nrows - 1) / p.rep + 1));
-  const int64_t own = (seen + BN - 1) / BN;
+  if (p.causal) seen = max(0, min(seen, it.slen - p.T + p.by_rep.div(it.row0 + it.nrows - 1) + 1));
+  const int own = (seen + BN - 1) / BN;
   if (p.stacked) {
     it.split = p.prefix_splits + part;
-    it.sb0 = (int)(own * part / p.own_splits);
-    it.sb1 = (int)(own * (part + 1) / p.own_splits);
+    deal(own, p.by_own_splits, part, it.sb0, it.sb1);
     return it;
   }
   it.split = part;
@@ -306,97 +368,103 @@ __device__ AttnItem attn_item(const AttnParams& p, int lane) {
   if (p.starts != nullptr) {
     for (int i = 1 + lane; i < p.G; i += 32) g += p.starts[i] <= it.b;
     g = __reduce_add_sync(0xffffffffu, g);
-  } else {
+  } else if (p.G > 1) {
     g = (int)((int64_t)it.b * p.G / p.B);
   }
   it.g = g;
   it.plen = clamp_len(p.prefix_lens, g, p.P);
-  const int64_t prefix = (it.plen + BN - 1) / BN, all = prefix + own;
-  const int64_t c0 = all * part / p.prefix_splits, c1 = all * (part + 1) / p.prefix_splits;
-  it.pb0 = (int)(c0 < prefix ? c0 : prefix), it.pb1 = (int)(c1 < prefix ? c1 : prefix);
-  it.sb0 = (int)(c0 < prefix ? 0 : c0 - prefix), it.sb1 = (int)(c1 < prefix ? 0 : c1 - prefix);
+  const int prefix = (it.plen + BN - 1) / BN;
+  int c0, c1;  // of the prefix's blocks and then the own ones
+  deal(prefix + own, p.by_prefix_splits, part, c0, c1);
+  it.pb0 = min(c0, prefix), it.pb1 = min(c1, prefix);
+  it.sb0 = max(0, c0 - prefix), it.sb1 = max(0, c1 - prefix);
   return it;
 }
 
 template <typename T, int DP, int NT>
 __global__ void __launch_bounds__(AttnCfg<DP, NT>::WARPS * 32, 1)
-    prefix_attention_kernel(const __grid_constant__ CUtensorMap tm_pk, const __grid_constant__ CUtensorMap tm_pv,
+    prefix_attention_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUtensorMap tm_pk, const __grid_constant__ CUtensorMap tm_pv,
                             const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CUtensorMap tm_v,
                             const AttnParams p) {
   using C = AttnCfg<DP, NT>;
-  constexpr int BN = C::BN, RING = C::RING;
+  constexpr int BN = C::BN, NB = C::NB, RING = C::RING;
   extern __shared__ uint8_t smem_raw[];
-  __shared__ __align__(8) uint64_t full[RING], empty[RING], s_full[2], p_ready[2], pv_done[NT], all_done;
+  // step[t][i % NB], completed once per block i: the scores of block i are there, and O
+  // holds the blocks up to i - NB.  NB further steps follow the last block's.
+  __shared__ __align__(8) uint64_t full[RING], empty[RING], step[NT][NB], p_ready[NT][NB], drained[NT], q_full[NT];
   __shared__ uint32_t tmem_holder;
   __shared__ AttnItem item_sh;
+  __shared__ float pair_sh[2][C::ROWS];  // a row's two threads: maxima, at the end sums
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  constexpr int kProducer = 4 * NT, kIssuer = 4 * NT + 1;
+  const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
+  constexpr int kProducer = 8 * NT, kIssuer = 8 * NT + 1;
 
-  griddep_enter();
-  if (warp == kProducer) {
-    const AttnItem it = attn_item<BN, C::ROWS>(p, lane);
-    if (lane == 0) item_sh = it;
-    if (lane == 0) {
-      prefetch_tensormap(&tm_pk);
-      prefetch_tensormap(&tm_pv);
-      prefetch_tensormap(&tm_k);
-      prefetch_tensormap(&tm_v);
-    }
-  }
-  if (threadIdx.x == 0) {
-    for (int i = 0; i < RING; ++i) {
-      mbar_init(&full[i], 1);
-      mbar_init(&empty[i], 1);
-    }
-    for (int i = 0; i < 2; ++i) {
-      mbar_init(&s_full[i], 1);
-      mbar_init(&p_ready[i], 4);
-    }
-    for (int i = 0; i < NT; ++i) mbar_init(&pv_done[i], 1);
-    mbar_init(&all_done, 1);
-    fence_barrier_init();
-  }
-  __syncthreads();
-  const AttnItem it = item_sh;
-  if (it.nrows <= 0) return;
+  // What needs no input comes before the wait for the kernel before.
   if (warp == kIssuer) {
     tmem_alloc(&tmem_holder, C::TMEM_COLS);
     tmem_relinquish();
   }
-  const int per_seq = p.T * p.rep;
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < RING; ++i) {
+      mbar_init(&full[i], 1);
+      mbar_init(&empty[i], NT);
+    }
+    for (int i = 0; i < NB * NT; ++i) {
+      mbar_init(&step[0][0] + i, 1);
+      mbar_init(&p_ready[0][0] + i, 8);
+    }
+    for (int i = 0; i < NT; ++i) {
+      mbar_init(&drained[i], 1);
+      mbar_init(&q_full[i], p.q_boxes ? 1 : 8);
+    }
+    fence_barrier_init();
+  }
+  if (warp == kProducer && lane == 0) {
+    prefetch_tensormap(&tm_q);
+    prefetch_tensormap(&tm_pk);
+    prefetch_tensormap(&tm_pv);
+    prefetch_tensormap(&tm_k);
+    prefetch_tensormap(&tm_v);
+  }
+  griddep_enter();
+  if (warp == kProducer) {
+    const AttnItem it = attn_item<BN, C::ROWS>(p, lane);
+    if (lane == 0) item_sh = it;
+  }
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = tmem_holder;
+  const AttnItem it = item_sh;
+  const int per_seq = p.T * p.rep;
   const int np = it.pb1 - it.pb0, nblk = np + it.sb1 - it.sb0;
-  // Ring positions of a block's K and V, in the order the issuer needs them.
-  auto k_pos = [&](int i) { return NT == 2 ? 2 * i : i == 0 ? 0 : 2 * i - 1; };
-  auto v_pos = [&](int i) { return NT == 2 ? 2 * i + 1 : i + 1 < nblk ? 2 * i + 2 : 2 * i + 1; };
+  // Ring positions, in the order the issuers need them: the first NB K, then V0 K(NB) V1
+  // K(NB + 1) ..., at the end the last NB V.
+  const int lead = min(NB, nblk), late = nblk - lead;
+  auto v_pos = [&](int i) { return lead + i + min(i, late); };
   uint8_t* ring = smem + C::Q_BYTES;
   bool ok = true;
 
   if (warp == kProducer) {
     if (lane == 0) {
+      if (p.q_boxes && nblk > 0) {
+        // Rows (token, head of the group) of a tile are a box of whole tokens; what lies
+        // behind the last row is another sequence's or nothing's, and no row that counts.
+        const int token = it.seq0 * p.T + p.by_rep.div(it.row0);
+        for (int t = 0; t < NT; ++t) {
+          mbar_arrive_expect_tx(&q_full[t], 128 * DP * 2);
+          for (int c = 0; c < DP / 64; ++c)
+            tma_load_4d(smem_u32(smem) + t * (128 * DP * 2) + c * (128 * 128), &tm_q, 64 * c, it.kv * p.rep,
+                        token + t * p.by_rep.div(128), 0, smem_u32(&q_full[t]));
+        }
+      }
       int issued = 0;
-      for (int pos = 0; pos < 2 * nblk && ok; ++pos) {
-        // pos -> which block, K or V
-        int i, is_v;
-        if (NT == 2) {
-          i = pos >> 1, is_v = pos & 1;
-        } else if (pos == 0) {
-          i = 0, is_v = 0;
-        } else if (pos == 2 * nblk - 1) {
-          i = nblk - 1, is_v = 1;
-        } else {
-          is_v = (pos & 1) == 0;
-          i = is_v ? pos / 2 - 1 : (pos + 1) / 2;
-        }
+      for (int pos = 0; pos < 2 * nblk; ++pos) {
+        const int q = pos - lead;  // from here on V and K take turns
+        const bool is_v = q >= 2 * late || (q >= 0 && (q & 1) == 0);
+        const int i = q < 0 ? pos : q >= 2 * late ? q - late : is_v ? q / 2 : NB + q / 2;
         const int slot = pos % RING;
-        if (pos >= RING && !mbar_wait(&empty[slot], (pos / RING - 1) & 1, kSiteAttn)) {
-          ok = false;
-          break;
-        }
+        if (pos >= RING && !mbar_wait(&empty[slot], (pos / RING - 1) & 1, kSiteAttn)) break;
         mbar_arrive_expect_tx(&full[slot], C::SLOT_BYTES);
         const bool prefix = i < np;
         const CUtensorMap* map = prefix ? (is_v ? &tm_pv : &tm_pk) : (is_v ? &tm_v : &tm_k);
@@ -410,222 +478,276 @@ __global__ void __launch_bounds__(AttnCfg<DP, NT>::WARPS * 32, 1)
       // Never leave the CTA with copies still landing in shared memory.
       for (int pos = issued > RING ? issued - RING : 0; pos < issued; ++pos)
         mbar_wait(&full[pos % RING], (pos / RING) & 1, kSiteAttn + 1);
+      for (int t = 0; p.q_boxes && nblk > 0 && t < NT; ++t) mbar_wait(&q_full[t], 0, kSiteAttn + 1);
     }
-  } else if (warp == kIssuer) {
-    if (nblk > 0) named_barrier_sync(1, (4 * NT + 1) * 32);  // Q is in shared memory
-    if (lane == 0 && nblk > 0) {
-      const uint32_t q0 = smem_u32(smem), r0 = smem_u32(ring);
-      auto wait_slot = [&](int pos) { return mbar_wait(&full[pos % RING], (pos / RING) & 1, kSiteAttn + 2); };
-      auto scores = [&](int t, int buffer, int pos) {  // S[buffer] = Q_t K^T
-        const uint32_t kb = r0 + (pos % RING) * C::SLOT_BYTES, qb = q0 + t * (128 * DP * 2);
+  } else if (warp >= kIssuer) {
+    // One issuing thread per row tile: it is held while its MMAs and commits go out, which
+    // the other tile's overlap.  The ring is walked in order and every operand is an
+    // increment of the one before: address arithmetic between two MMAs is time the tensor
+    // core waits.
+    const int t = warp - kIssuer;
+    if (nblk > 0 && lane == 0) {
+      const uint64_t q_desc = smem_desc_sw128(smem_u32(smem) + t * (128 * DP * 2));
+      const uint64_t k_desc0 = smem_desc_sw128(smem_u32(ring)), v_desc0 = smem_desc_mn_sw128(smem_u32(ring), BN);
+      constexpr uint32_t kSlotStep = C::SLOT_BYTES >> 4;
+      const uint32_t o_col = tmem + C::O_COL + t * DP, s_col = tmem + C::S_COL + t * NB * BN;
+      int slot = 0;
+      uint32_t lap = 0;
+      auto next = [&] {
+        if (++slot == RING) slot = 0, lap ^= 1;
+      };
+      auto scores = [&](uint32_t s_at) {  // S = Q K^T
+        const uint64_t k_desc = k_desc0 + (uint32_t)slot * kSlotStep;
 #pragma unroll
         for (int k = 0; k < DP / 16; ++k)
-          mma16_ss(tmem + C::S_COL + buffer * BN, smem_desc_sw128(qb + (k / 4) * (128 * 128) + (k % 4) * 32),
-                   smem_desc_sw128(kb + (k / 4) * (BN * 128) + (k % 4) * 32), idesc_16<T>(BN, false), k > 0);
+          mma16_ss(s_at, q_desc + (k / 4) * (128 * 128 / 16) + (k % 4) * 2,
+                   k_desc + (k / 4) * (BN * 128 / 16) + (k % 4) * 2, idesc_16<T>(BN, false), k > 0);
       };
-      auto values = [&](int t, int buffer, int pos, bool first) {  // O_t += P[buffer] V
-        const uint32_t vb = r0 + (pos % RING) * C::SLOT_BYTES;
-#pragma unroll
-        for (int k = 0; k < BN / 16; ++k)
-          mma16_ts(tmem + C::O_COL + t * DP, tmem + C::S_COL + buffer * BN + k * 8,
-                   smem_desc_mn_sw128(vb + k * 2048, BN), idesc_16<T>(DP, true), !first || k > 0);
-      };
-      ok = wait_slot(k_pos(0));
-      if (ok) {
+      ok = mbar_wait(&q_full[t], 0, kSiteAttn + 2);
+      for (int i = 0; i < lead && ok; ++i) {
+        if (!(ok = mbar_wait(&full[slot], lap, kSiteAttn + 2))) break;
         tc_fence_after();
-        for (int t = 0; t < NT; ++t) {
-          scores(t, t, k_pos(0));
-          mma_commit(&s_full[t]);
-        }
-        mma_commit(&empty[k_pos(0) % RING]);
+        scores(s_col + i * BN);
+        mma_commit(&step[t][i]);
+        mma_commit(&empty[slot]);
+        next();
       }
+      int buffer = 0;
+      uint32_t turn = 0;  // p_ready's phase
       for (int i = 0; i < nblk && ok; ++i) {
-        if constexpr (NT == 1) {
-          if (i + 1 < nblk) {
-            // The other score buffer: its P was consumed by the product issued before.
-            if (!(ok = wait_slot(k_pos(i + 1)))) break;
-            tc_fence_after();
-            scores(0, (i + 1) & 1, k_pos(i + 1));
-            mma_commit(&s_full[(i + 1) & 1]);
-            mma_commit(&empty[k_pos(i + 1) % RING]);
-          }
-          ok = wait_slot(v_pos(i)) && mbar_wait(&p_ready[i & 1], (i >> 1) & 1, kSiteAttn + 3);
-          if (!ok) break;
+        const uint64_t v_desc = v_desc0 + (uint32_t)slot * kSlotStep;
+        const uint32_t s_at = s_col + buffer * BN;
+        ok = mbar_wait(&full[slot], lap, kSiteAttn + 2) && mbar_wait(&p_ready[t][buffer], turn, kSiteAttn + 3);
+        if (!ok) break;
+        tc_fence_after();
+#pragma unroll
+        for (int k = 0; k < BN / 16; ++k)  // O += P V; each half of the keys has its p over its own scores
+          mma16_ts(o_col, s_at + (k / (BN / 32)) * (BN / 2) + (k % (BN / 32)) * 8, v_desc + k * (2048 / 16),
+                   idesc_16<T>(DP, true), i > 0 || k > 0);
+        mma_commit(&empty[slot]);
+        next();
+        if (i + NB < nblk) {
+          if (!(ok = mbar_wait(&full[slot], lap, kSiteAttn + 2))) break;
           tc_fence_after();
-          values(0, i & 1, v_pos(i), i == 0);
-          mma_commit(&empty[v_pos(i) % RING]);
-          mma_commit(&pv_done[0]);
+          scores(s_at);  // over the p that O just took
+          mma_commit(&step[t][buffer]);
+          mma_commit(&empty[slot]);
+          next();
         } else {
-          for (int t = 0; t < NT && ok; ++t) {
-            ok = (t > 0 || wait_slot(v_pos(i))) && mbar_wait(&p_ready[t], i & 1, kSiteAttn + 3);
-            if (!ok) break;
-            tc_fence_after();
-            values(t, t, v_pos(i), i == 0);
-            if (t == NT - 1) mma_commit(&empty[v_pos(i) % RING]);
-            mma_commit(&pv_done[t]);
-            if (i + 1 < nblk) {
-              if (t == 0 && !(ok = wait_slot(k_pos(i + 1)))) break;
-              tc_fence_after();
-              scores(t, t, k_pos(i + 1));
-              mma_commit(&s_full[t]);
-              if (t == NT - 1) mma_commit(&empty[k_pos(i + 1) % RING]);
-            }
-          }
+          mma_commit(&step[t][buffer]);
         }
+        if (++buffer == NB) buffer = 0, turn ^= 1;
       }
-      mma_commit(&all_done);
-      mbar_wait(&all_done, 0, kSiteAttn + 4);  // nothing in flight reads shared memory after this
+      if (ok) {
+        const int last = nblk - 1 + NB;
+        mbar_wait(&step[t][last % NB], (last / NB) & 1, kSiteAttn + 4);
+      } else {
+        // A wait ran out: the outputs are void, but nothing may read shared memory after the CTA.
+        mma_commit(&drained[t]);
+        mbar_wait(&drained[t], 0, kSiteAttn + 4);
+      }
     }
   } else {
-    const int t = warp >> 2;                      // row tile
-    const int my = threadIdx.x;                   // row of the CTA
+    // Two threads share a row, each with half the keys of a block: two warps a tile on each
+    // SM sub-core hide one another's latencies.
+    const int t = warp >> 3, half = (warp >> 2) & 1;
+    const int my = t * 128 + (warp & 3) * 32 + lane;  // row of the CTA
+    const int pair_bar = 1 + t * 4 + (warp & 3);      // the two warps of these 32 rows
     const uint32_t lanes = (uint32_t)(warp & 3) << 21;  // this warp's 32 tensor-memory lanes
-    const int idx = it.row0 + my, b = it.seq0 + idx / per_seq, r = idx % per_seq;
-    const int tok = r / p.rep, head = it.kv * p.rep + r % p.rep;
+    int b = it.row0 + my;
+    int head = p.by_per_seq.split(b);  // row of its sequence: token * rep + head of the group
+    int tok = head;
+    head = it.kv * p.rep + p.by_rep.split(tok);
+    b += it.seq0;
     const bool live = my < it.nrows;
-    if (nblk > 0) {
-      // Q, K-major, 128-byte swizzled, in column tiles of 64; a warp brings its 32 rows,
-      // rows and columns past the end are zeros.
+    if (nblk > 0 && !p.q_boxes) {
+      // Q as the boxes would bring it: K-major, 128-byte swizzled, in column tiles of 64; a
+      // warp brings half of each of its 32 rows; rows and columns past the end are zeros.
       constexpr int CH = DP / 8;  // 16-byte pieces of a row
       const T* q = reinterpret_cast<const T*>(p.q);
       const int64_t mine = live ? b * p.q_b + tok * p.q_t + head * p.q_h : -1;
-#pragma unroll 4
-      for (int c = lane; c < 32 * CH; c += 32) {
+      for (int c = half * 32 + lane; c < 32 * CH; c += 64) {
         const int rr = c / CH, x = c % CH;
         const int64_t at = __shfl_sync(0xffffffffu, mine, rr);
-        uint4 u = make_uint4(0, 0, 0, 0);
-        if (at >= 0 && 8 * x < p.D) u = *reinterpret_cast<const uint4*>(q + at + 8 * x);
+        const bool there = at >= 0 && 8 * x < p.D;
         const int row = (warp & 3) * 32 + rr;
-        uint8_t* dst = smem + t * (128 * DP * 2) + (x >> 3) * (128 * 128) + row * 128;
-        *reinterpret_cast<uint4*>(dst + (((x & 7) ^ (row & 7)) << 4)) = u;
+        copy16_or_zero(smem_u32(smem) + t * (128 * DP * 2) + (x >> 3) * (128 * 128) + row * 128 + (((x & 7) ^ (row & 7)) << 4),
+                       q + (there ? at + 8 * x : 0), there);
       }
+      copy16_wait();
       fence_proxy_async_smem();
-      named_barrier_sync(1, (4 * NT + 1) * 32);
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&q_full[t]);
     }
     int own_end = it.slen;  // own keys this row sees
     if (p.causal) own_end = max(0, min(it.slen, it.slen - p.T + tok + 1));
+    const bool idle = t * 128 + (warp & 3) * 32 >= it.nrows;
     float m = -INFINITY, l = 0.f;
     const uint32_t o_addr = tmem + lanes + C::O_COL + t * DP;
-    for (int i = 0; i < nblk && ok; ++i) {
-      const int buffer = NT == 1 ? i & 1 : t;
-      const bool prefix = i < np;
-      const int key = (prefix ? it.pb0 + i : it.sb0 + i - np) * BN;
-      const int end = (prefix ? it.plen : own_end) - key;  // keys of the block this row sees
-      // Cache rows past the length may hold anything, and p = 0 would not hide a NaN.
-      const int filled = (prefix ? it.plen : it.slen) - key;
-      if (t == 0 && filled < BN && key + filled < (prefix ? p.P : p.S)) {
-        const int pos = v_pos(i);
-        ok = mbar_wait(&full[pos % RING], (pos / RING) & 1, kSiteAttn + 5);
-        uint8_t* v = ring + (pos % RING) * C::SLOT_BYTES;
-        const int gone = BN - filled;
-        for (int c = my; c < gone * (DP / 8); c += 128) {
-          const int r = filled + c % gone, x = c / gone;
-          *reinterpret_cast<uint4*>(v + (x >> 3) * (BN * 128) + r * 128 + (x & 7) * 16) = make_uint4(0, 0, 0, 0);
+    constexpr int HALF = BN / 2;  // keys of a block that are this thread's
+    static_assert(HALF == 32, "a thread's scores are one load");
+    const uint32_t s_addr0 = tmem + lanes + C::S_COL + t * NB * BN + half * HALF;
+    // Blocks that hold keys some row of the warp does not see: the prefix's last if it is
+    // not full, and the own ones from own_mask on.
+    const int mask_prefix = np > 0 && (int64_t)it.pb1 * BN > it.plen ? np - 1 : -1;
+    const int own_mask = np + max(0, (int)__reduce_min_sync(0xffffffffu, own_end) / BN - it.sb0);
+    int buffer = 0;
+    uint32_t turn = 0;
+    for (int i = 0; i < nblk; ++i) {
+      const bool masked = i == mask_prefix || i >= own_mask;
+      int end = BN;  // keys of this half that the row sees
+      if (masked) {
+        const bool prefix = i < np;
+        const int key = (prefix ? it.pb0 + i : it.sb0 + i - np) * BN;
+        end = (prefix ? it.plen : own_end) - key - half * HALF;
+        // Cache rows past the length may hold anything, and p = 0 would not hide a NaN.
+        // (Each tile clears them before its own product; the second time changes nothing.)
+        const int filled = (prefix ? it.plen : it.slen) - key;
+        if (filled < BN && key + filled < (prefix ? p.P : p.S)) {
+          const int pos = v_pos(i);
+          ok = ok && mbar_wait(&full[pos % RING], (pos / RING) & 1, kSiteAttn + 5);
+          uint8_t* v = ring + (pos % RING) * C::SLOT_BYTES;
+          const int gone = BN - filled;
+          for (int c = threadIdx.x & 255; c < gone * (DP / 8); c += 256) {
+            const int rr = filled + c % gone, col = c / gone;
+            *reinterpret_cast<uint4*>(v + (col >> 3) * (BN * 128) + rr * 128 + (col & 7) * 16) = make_uint4(0, 0, 0, 0);
+          }
+          fence_proxy_async_smem();
         }
-        fence_proxy_async_smem();
       }
-      ok = mbar_wait(&s_full[buffer], NT == 1 ? (i >> 1) & 1 : i & 1, kSiteAttn + 6) && ok;
-      if (!(ok = __all_sync(0xffffffffu, ok))) break;
-      tc_fence_after();
-      const uint32_t s_addr = tmem + lanes + C::S_COL + buffer * BN;
-      float s[BN];
-#pragma unroll
-      for (int c = 0; c < BN / 32; ++c) tmem_ld32(s_addr + 32 * c, reinterpret_cast<uint32_t(&)[32]>(s[32 * c]));
-      tmem_wait_ld();
-      if (!__all_sync(0xffffffffu, end >= BN)) {
-#pragma unroll
-        for (int j = 0; j < BN; ++j) s[j] = j < end ? s[j] : -INFINITY;
-      }
-      float top[4] = {s[0], s[1], s[2], s[3]};
-#pragma unroll
-      for (int j = 4; j < BN; ++j) top[j & 3] = fmaxf(top[j & 3], s[j]);
-      const float mx = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])) * p.scale;
-      const bool grown = mx - m > kRescale;  // m = -inf: O and l are zero, only m is set
-      const bool rescale = __any_sync(0xffffffffu, grown && m != -INFINITY);
-      // Every phase of pv_done is waited for, here or below: a parity tells only
-      // neighbouring phases apart.
-      if (rescale) {
-        const float f = grown && m != -INFINITY ? exp2_approx(m - mx) : 1.f;
-        ok = mbar_wait(&pv_done[t], (i - 1) & 1, kSiteAttn + 7);
-        if (!(ok = __all_sync(0xffffffffu, ok))) break;
+      ok = ok && mbar_wait(&step[t][buffer], turn, kSiteAttn + 6);
+      ok = __all_sync(0xffffffffu, ok);
+      const uint32_t s_addr = s_addr0 + buffer * BN;
+      uint32_t x[32], pk[16];
+      if (!idle) {
         tc_fence_after();
+        tmem_ld32(s_addr, x);
+      }
+      if (!idle) {  // else: whatever these rows' p hold stays in them
+        tmem_wait_ld32(x);
+        if (masked) {
 #pragma unroll
-        for (int c = 0; c < DP / 32; ++c) {
-          uint32_t o[32];
-          tmem_ld32(o_addr + 32 * c, o);
-          tmem_wait_ld();
-#pragma unroll
-          for (int j = 0; j < 32; ++j) o[j] = __float_as_uint(__uint_as_float(o[j]) * f);
-          tmem_st32(o_addr + 32 * c, o);
+          for (int j = 0; j < 32; ++j) x[j] = j < end ? x[j] : 0xff800000u;
         }
-        l *= f;
-      }
-      if (grown) m = mx;
-      const float ref = m == -INFINITY ? 0.f : m;
-      const float2 c2 = make_float2(p.scale, p.scale), r2 = make_float2(-ref, -ref);
-      float2 sum[2] = {};
-      uint32_t pk[BN / 2];
+        // The exponentials are taken against the maximum so far while the block's own is
+        // found beside them.  Only where that is more than 2^8 above (or there is none yet)
+        // O and l are brought to the new maximum and the exponentials taken again.
+        for (bool again = false;; again = true) {
+          const float ref = m == -INFINITY ? 0.f : m;
+          const float2 c2 = make_float2(p.scale, p.scale), r2 = make_float2(-ref, -ref);
+          float top[2] = {-INFINITY, -INFINITY};
+          float2 add[2] = {};
 #pragma unroll
-      for (int j = 0; j < BN / 2; ++j) {
-        float2 e = ffma2(make_float2(s[2 * j], s[2 * j + 1]), c2, r2);
-        e.x = exp2_approx(e.x), e.y = exp2_approx(e.y);
-        sum[j & 1] = fadd2(sum[j & 1], e);
-        pk[j] = pack16<T>(e.x, e.y);
-      }
+          for (int j = 0; j < 16; ++j) {
+            const float2 v = make_float2(__uint_as_float(x[2 * j]), __uint_as_float(x[2 * j + 1]));
+            top[j & 1] = fmaxf(top[j & 1], fmaxf(v.x, v.y));
+            float2 e = ffma2(v, c2, r2);
+            e.x = exp2_approx(e.x), e.y = exp2_approx(e.y);
+            add[j & 1] = fadd2(add[j & 1], e);
+            pk[j] = pack16<T>(e.x, e.y);
+          }
+          const float mx = fmaxf(top[0], top[1]) * p.scale;
+          // (A warp whose wait ran out goes on without data, so that no barrier lacks it.)
+          if (again || named_barrier_and(pair_bar, 64, !(mx - m > kRescale))) {
+            add[0] = fadd2(add[0], add[1]);
+            l += add[0].x + add[0].y;
+            break;
+          }
+          pair_sh[half][my] = mx;
+          named_barrier_sync(pair_bar, 64);
+          const float both = fmaxf(mx, pair_sh[half ^ 1][my]);
+          const bool grown = both - m > kRescale;
+          if (i > 0 && __any_sync(0xffffffffu, grown && m != -INFINITY)) {  // m = -inf: O and l are zero
+            const float f = grown && m != -INFINITY ? exp2_approx(m - both) : 1.f;
+            // The step that tells that O holds the block before this one.
+            const int s = i - 1 + NB;
+            ok = ok && mbar_wait(&step[t][s % NB], (s / NB) & 1, kSiteAttn + 7);
+            ok = __all_sync(0xffffffffu, ok);
+            tc_fence_after();
+#pragma unroll 1
+            for (int d = half * (DP / 2); d < (half + 1) * (DP / 2); d += 32) {
+              uint32_t o[32];
+              tmem_ld32(o_addr + d, o);
+              tmem_wait_ld32(o);
 #pragma unroll
-      for (int c = 0; c < BN / 64; ++c) tmem_st32(s_addr + 32 * c, pk + 32 * c);
-      l += (sum[0].x + sum[0].y) + (sum[1].x + sum[1].y);
-      tmem_wait_st();
-      if (i > 0 && !rescale) ok = mbar_wait(&pv_done[t], (i - 1) & 1, kSiteAttn + 7);
-      if (!(ok = __all_sync(0xffffffffu, ok))) break;
-      tc_fence_before();
+              for (int j = 0; j < 32; ++j) o[j] = __float_as_uint(__uint_as_float(o[j]) * f);
+              tmem_st32(o_addr + d, o);
+            }
+            l *= f;
+          }
+          if (grown) m = both;
+        }
+      }
+      if (!idle) {
+        tmem_st16(s_addr, pk);  // two to a column, over this half's scores
+        tmem_wait_st();
+        tc_fence_before();
+      }
       __syncwarp();
-      if (lane == 0) mbar_arrive(&p_ready[buffer]);
+      if (lane == 0) mbar_arrive(&p_ready[t][buffer]);
+      if (++buffer == NB) buffer = 0, turn ^= 1;
     }
-    if (nblk > 0 && ok) ok = mbar_wait(&pv_done[t], (nblk - 1) & 1, kSiteAttn + 8);
+    if (nblk > 0 && ok) {
+      const int last = nblk - 1 + NB;
+      ok = mbar_wait(&step[t][last % NB], (last / NB) & 1, kSiteAttn + 8);
+    }
     ok = __all_sync(0xffffffffu, ok);
-    if (ok) {
+    pair_sh[half][my] = l;
+    named_barrier_sync(pair_bar, 64);
+    l += pair_sh[half ^ 1][my];
+    if (ok && !idle) {
+      // O from tensor memory by rows (a thread each), to global memory by lines: through
+      // this warp's share of the tile's Q, which nothing reads any more.  Straight from a
+      // thread per row, every 16 bytes of a store would be a memory sector of their own.
       tc_fence_after();
-      const int64_t row = ((int64_t)b * p.T + tok) * p.H + head;
-      if (p.splits == 1) {
-        const float inv = l == 0.f ? 0.f : 1.f / l;
-        T* dst = reinterpret_cast<T*>(p.out) + row * p.D;
+      constexpr int CH = DP / 16;  // 16-byte pieces that a row has in the warp's share
+      uint8_t* stage = smem + t * (128 * DP * 2) + (warp & 7) * (32 * DP);
+      const auto piece = [&](int r, int j) {
+        return reinterpret_cast<uint4*>(stage + r * DP + ((j ^ (DP > 64 ? r & 7 : r >> 1 & 3)) << 4));
+      };
+      const int row = (b * p.T + tok) * p.H + head;
+      const int64_t rows = (int64_t)p.B * p.T * p.H;
+      const float inv = l == 0.f ? 0.f : 1.f / l;
+      if (p.splits > 1 && live && half == 0) p.ml[it.split * rows + row] = make_float2(m, nblk > 0 ? l : 0.f);
+      // fp32 parts take two rounds of DP / 4 columns, finished rows one of DP / 2.
+      for (int round = 0; round < (p.splits == 1 ? 1 : nblk > 0 ? 2 : 0); ++round) {
+        const int col = half * (DP / 2) + round * (DP / 4);
+        if (p.splits == 1) {
 #pragma unroll
-        for (int c = 0; c < DP / 32; ++c) {
-          if (32 * c >= p.D) break;
-          uint32_t o[32];
-          if (nblk > 0) tmem_ld32(o_addr + 32 * c, o);
-          tmem_wait_ld();
-          if (!live) continue;
+          for (int c = 0; c < DP / 2; c += 32) {
+            uint32_t o[32], w[16];
+            if (nblk > 0) tmem_ld32(o_addr + col + c, o);
+            tmem_wait_ld32(o);
 #pragma unroll
-          for (int j = 0; j < 32; j += 8) {
-            if (32 * c + j >= p.D) break;
-            uint32_t w[4];
+            for (int e = 0; e < 16; ++e)
+              w[e] = l == 0.f ? 0u : pack16<T>(__uint_as_float(o[2 * e]) * inv, __uint_as_float(o[2 * e + 1]) * inv);
 #pragma unroll
-            for (int e = 0; e < 4; ++e)
-              w[e] = l == 0.f ? 0u
-                              : pack16<T>(__uint_as_float(o[j + 2 * e]) * inv, __uint_as_float(o[j + 2 * e + 1]) * inv);
-            *reinterpret_cast<uint4*>(dst + 32 * c + j) = make_uint4(w[0], w[1], w[2], w[3]);
+            for (int e = 0; e < 4; ++e) *piece(lane, c / 8 + e) = make_uint4(w[4 * e], w[4 * e + 1], w[4 * e + 2], w[4 * e + 3]);
+          }
+        } else {
+#pragma unroll
+          for (int c = 0; c < DP / 4; c += 16) {
+            uint32_t o[16];
+            tmem_ld16(o_addr + col + c, o);
+            tmem_wait_ld16(o);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) *piece(lane, c / 4 + e) = make_uint4(o[4 * e], o[4 * e + 1], o[4 * e + 2], o[4 * e + 3]);
           }
         }
-      } else {
-        const int64_t rows = (int64_t)p.B * p.T * p.H;
-        if (live) p.ml[it.split * rows + row] = make_float2(m, nblk > 0 ? l : 0.f);
-        if (nblk > 0) {
-          float* dst = p.o_part + (it.split * rows + row) * p.D;
-#pragma unroll
-          for (int c = 0; c < DP / 32; ++c) {
-            if (32 * c >= p.D) break;
-            uint32_t o[32];
-            tmem_ld32(o_addr + 32 * c, o);
-            tmem_wait_ld();
-            if (!live || l == 0.f) continue;
-#pragma unroll
-            for (int j = 0; j < 32; j += 4)
-              if (32 * c + j < p.D)
-                *reinterpret_cast<uint4*>(dst + 32 * c + j) = make_uint4(o[j], o[j + 1], o[j + 2], o[j + 3]);
-          }
+        __syncwarp();
+        const int per = p.splits == 1 ? 8 : 4;  // columns of a piece
+#pragma unroll 8
+        for (int c = lane; c < 32 * CH; c += 32) {
+          const int r = c / CH, j = c % CH;
+          const int at = __shfl_sync(0xffffffffu, live ? row : -1, r), d = col + j * per;
+          if (at < 0 || d >= p.D) continue;
+          const uint4 u = *piece(r, j);
+          if (p.splits == 1)
+            *reinterpret_cast<uint4*>(reinterpret_cast<T*>(p.out) + (int64_t)at * p.D + d) = u;
+          else
+            *reinterpret_cast<uint4*>(p.o_part + (it.split * rows + at) * p.D + d) = u;
         }
+        __syncwarp();
       }
     }
     tc_fence_before();
@@ -634,6 +756,8 @@ __global__ void __launch_bounds__(AttnCfg<DP, NT>::WARPS * 32, 1)
   if (warp == kIssuer) tmem_dealloc(tmem, C::TMEM_COLS);
 }
 
+constexpr int kMostSplits = 96;  // parts of a row
+
 // Joins the parts of a row: one warp per row, D a multiple of 8.
 template <typename T>
 __global__ void __launch_bounds__(128) prefix_attention_join_kernel(const AttnParams p) {
@@ -641,23 +765,39 @@ __global__ void __launch_bounds__(128) prefix_attention_join_kernel(const AttnPa
   const int lane = threadIdx.x & 31;
   const int64_t rows = (int64_t)p.B * p.T * p.H, row = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 5);
   if (row >= rows) return;
-  float top = -INFINITY;
-  for (int s = lane; s < p.splits; s += 32) top = fmaxf(top, p.ml[s * rows + row].x);
+  // Weights first, a part per lane (kMostSplits of them): the loads of O then depend on
+  // nothing and go out together.  A part that saw no key has l = 0 and no O.
+  float2 ml[kMostSplits / 32];
+  float top = -INFINITY, total = 0.f;
+#pragma unroll
+  for (int i = 0; i < kMostSplits / 32; ++i) {
+    const int s = lane + 32 * i;
+    ml[i] = s < p.splits ? p.ml[s * rows + row] : make_float2(-INFINITY, 0.f);
+    top = fmaxf(top, ml[i].x);
+  }
 #pragma unroll
   for (int d = 16; d; d >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
-  float total = 0.f;
-  float2 o[4] = {};
-  for (int s = 0; s < p.splits; ++s) {
-    const float2 ml = p.ml[s * rows + row];
-    if (ml.y == 0.f) continue;  // this part saw no key; its O was not written
-    const float w = exp2_approx(ml.x - top);
-    total = fmaf(w, ml.y, total);
-    const float* src = p.o_part + (s * rows + row) * p.D;
+  float weight[kMostSplits / 32];
 #pragma unroll
-    for (int c = 0; c < 4; ++c) {
-      const int d = 64 * c + 2 * lane;
-      if (d < p.D) {
-        const float2 a = *reinterpret_cast<const float2*>(src + d);
+  for (int i = 0; i < kMostSplits / 32; ++i) {
+    weight[i] = ml[i].y == 0.f ? 0.f : exp2_approx(ml[i].x - top);
+    total = fmaf(weight[i], ml[i].y, total);
+  }
+#pragma unroll
+  for (int d = 16; d; d >>= 1) total += __shfl_xor_sync(0xffffffffu, total, d);
+  float2 o[4] = {};
+#pragma unroll
+  for (int i = 0; i < kMostSplits / 32; ++i) {
+    const int count = min(32, p.splits - 32 * i);
+#pragma unroll 4
+    for (int s = 0; s < count; ++s) {
+      const float w = __shfl_sync(0xffffffffu, weight[i], s);
+      const bool some = __shfl_sync(0xffffffffu, ml[i].y, s) != 0.f;
+      const float* src = p.o_part + ((32 * i + s) * rows + row) * p.D;
+#pragma unroll
+      for (int c = 0; c < 4; ++c) {
+        const int d = 64 * c + 2 * lane;
+        const float2 a = some && d < p.D ? *reinterpret_cast<const float2*>(src + d) : make_float2(0.f, 0.f);
         o[c] = ffma2(make_float2(w, w), a, o[c]);
       }
     }
@@ -687,14 +827,15 @@ AttnPlan attn_plan(int64_t B, int64_t T, int64_t H, int64_t KV, int64_t D, int64
   AttnPlan best = {};
   int64_t best_cost = INT64_MAX;
   const int64_t rep = H / KV, per_seq = T * rep;
-  const int dp = D <= 64 ? 64 : D <= 128 ? 128 : 256, bn = dp > 128 ? 64 : 128;
-  const int64_t pb = ceil_div(P, bn), ob = ceil_div(S, bn);
+  const int dp = D <= 64 ? 64 : D <= 128 ? 128 : 256;
   constexpr int64_t kJoin = 3, kStart = 2;  // in blocks: joining parts; a CTA's prologue and epilogue
   for (int stacked = 0; stacked < 2; ++stacked) {
     if (stacked && (P == 0 || B == G)) continue;  // nothing to stack
     const int64_t rows = stacked ? ceil_div(B, G) * per_seq : per_seq;
     const int nt = dp <= 128 && rows > 128 ? 2 : 1;
     const int64_t tile = 128 * nt;
+    const int bn = 64;  // AttnCfg::BN
+    const int64_t pb = ceil_div(P, bn), ob = ceil_div(S, bn);
     AttnPlan c = {};
     c.dp = dp, c.nt = nt, c.bn = bn, c.stacked = stacked;
     c.tiles_per_seq = (int)ceil_div(per_seq, tile);
@@ -739,16 +880,18 @@ bool attn_sizes_ok(int64_t B, int64_t T, int64_t H, int64_t KV, int64_t D, int64
          B * T * H <= kMost;
 }
 
-// [n, rows, heads, D] with D contiguous -> boxes of 64 columns x bn rows of one head.
-int encode_cache(CUtensorMap* map, int dtype, const void* base, int64_t D, int64_t heads, int64_t rows, int64_t n,
-                 int64_t sh, int64_t sr, int64_t sn, int bn) {
-  const cuuint64_t dims[4] = {(cuuint64_t)D, (cuuint64_t)heads, (cuuint64_t)rows, (cuuint64_t)n};
-  const cuuint64_t strides[3] = {(cuuint64_t)(sh * 2), (cuuint64_t)(sr * 2), (cuuint64_t)(sn * 2)};
-  const cuuint32_t box[4] = {64, 1, (cuuint32_t)bn, 1};
+// [n, rows, heads, D] with D contiguous (extents and strides from the inside out) -> boxes
+// of 64 columns x box[0] heads x box[1] rows, 128-byte swizzled.
+int encode_rows(CUtensorMap* map, int dtype, const void* base, const int64_t (&extent)[4], const int64_t (&stride)[3],
+                const int (&box)[3]) {
+  cuuint64_t dims[4], strides[3];
+  cuuint32_t boxes[4] = {64, (cuuint32_t)box[0], (cuuint32_t)box[1], (cuuint32_t)box[2]};
+  for (int i = 0; i < 4; ++i) dims[i] = (cuuint64_t)extent[i];
+  for (int i = 0; i < 3; ++i) strides[i] = (cuuint64_t)stride[i] * 2;
   const cuuint32_t estr[4] = {1, 1, 1, 1};
   const CUresult r = tensor_map_encoder()(
       map, dtype == ACTUNE_DTYPE_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 4,
-      const_cast<void*>(base), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+      const_cast<void*>(base), dims, strides, boxes, estr, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
       CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   return r == CUDA_SUCCESS ? ACTUNE_OK : ACTUNE_ERR_CUDA;
 }
@@ -761,16 +904,16 @@ bool map_stride(int64_t* stride, int64_t extent) {
 }
 
 template <typename T, int DP, int NT>
-cudaError_t launch_attn(const CUtensorMap (&m)[4], const AttnParams& p, int64_t items, cudaStream_t stream) {
+cudaError_t launch_attn(const CUtensorMap (&m)[5], const AttnParams& p, int64_t items, cudaStream_t stream) {
   using C = AttnCfg<DP, NT>;
   const cudaError_t e = ensure_smem_limit<prefix_attention_kernel<T, DP, NT>>(C::SMEM);
   if (e != cudaSuccess) return e;
   return launch_pdl(prefix_attention_kernel<T, DP, NT>, dim3((unsigned)items), C::WARPS * 32, C::SMEM, stream, m[0],
-                    m[1], m[2], m[3], p);
+                    m[1], m[2], m[3], m[4], p);
 }
 
 template <typename T>
-cudaError_t dispatch_attn(const CUtensorMap (&m)[4], const AttnParams& p, const AttnPlan& c, cudaStream_t stream) {
+cudaError_t dispatch_attn(const CUtensorMap (&m)[5], const AttnParams& p, const AttnPlan& c, cudaStream_t stream) {
   cudaError_t e;
   if (c.dp == 256) e = launch_attn<T, 256, 1>(m, p, c.items, stream);
   else if (c.dp == 128) e = c.nt == 2 ? launch_attn<T, 128, 2>(m, p, c.items, stream) : launch_attn<T, 128, 1>(m, p, c.items, stream);
@@ -850,18 +993,28 @@ int actune_prefix_attention(const actune_prefix_attention_args* a, void* stream)
   p.prefix_splits = c.prefix_splits, p.own_splits = c.own_splits, p.splits = c.splits;
   p.ml = reinterpret_cast<float2*>(reinterpret_cast<uint8_t*>(a->workspace) + (size_t)c.splits * rows * p.D * 4);
   p.o_part = reinterpret_cast<float*>(a->workspace);
-  CUtensorMap maps[4] = {};
+  p.by_prefix_tiles.set(c.prefix_tiles > 0 ? c.prefix_tiles : 1), p.by_kv.set(p.KV);
+  p.by_own_tiles.set((int64_t)p.B * c.tiles_per_seq), p.by_tiles_per_seq.set(c.tiles_per_seq);
+  p.by_per_seq.set((int64_t)p.T * p.rep), p.by_rep.set(p.rep);
+  p.by_prefix_splits.set(c.prefix_splits > 0 ? c.prefix_splits : 1), p.by_own_splits.set(c.own_splits > 0 ? c.own_splits : 1);
+  CUtensorMap maps[5] = {};
   int st = ACTUNE_OK;
-  if (a->P > 0) {
-    st = encode_cache(&maps[0], a->dtype, a->prefix_k, a->D, a->KV, a->P, a->G, pk_s[0], pk_s[1], pk_s[2], c.bn);
-    if (st == ACTUNE_OK)
-      st = encode_cache(&maps[1], a->dtype, a->prefix_v, a->D, a->KV, a->P, a->G, pv_s[0], pv_s[1], pv_s[2], c.bn);
+  // Queries as [B * T tokens, H, D], where the tokens are evenly spaced and a tile of 128
+  // rows is whole tokens.
+  int64_t q_s[3] = {a->q_h, a->T > 1 ? a->q_t : a->q_b, 0};
+  if (128 % p.rep == 0 && (a->B == 1 || a->T == 1 || a->q_b == a->T * a->q_t) && map_stride(&q_s[0], a->H) &&
+      map_stride(&q_s[1], a->B * a->T)) {
+    p.q_boxes = 1;
+    st = encode_rows(&maps[0], a->dtype, a->q, {a->D, a->H, a->B * a->T, 1}, {q_s[0], q_s[1], 256}, {p.rep, 128 / p.rep, 1});
   }
-  if (a->S > 0 && st == ACTUNE_OK) {
-    st = encode_cache(&maps[2], a->dtype, a->k, a->D, a->KV, a->S, a->B, k_s[0], k_s[1], k_s[2], c.bn);
-    if (st == ACTUNE_OK)
-      st = encode_cache(&maps[3], a->dtype, a->v, a->D, a->KV, a->S, a->B, v_s[0], v_s[1], v_s[2], c.bn);
-  }
+  const auto cache = [&](int i, const void* base, int64_t rows, int64_t n, const int64_t (&str)[3]) {
+    if (rows > 0 && st == ACTUNE_OK)
+      st = encode_rows(&maps[i], a->dtype, base, {a->D, a->KV, rows, n}, {str[0], str[1], str[2]}, {1, c.bn, 1});
+  };
+  cache(1, a->prefix_k, a->P, a->G, pk_s);
+  cache(2, a->prefix_v, a->P, a->G, pv_s);
+  cache(3, a->k, a->S, a->B, k_s);
+  cache(4, a->v, a->S, a->B, v_s);
   if (st != ACTUNE_OK) return st;
   return serving_status(a->dtype == ACTUNE_DTYPE_BF16 ? dispatch_attn<__nv_bfloat16>(maps, p, c, cs)
                                                       : dispatch_attn<__half>(maps, p, c, cs));
