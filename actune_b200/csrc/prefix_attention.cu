@@ -272,13 +272,14 @@ struct AttnCfg {
   static constexpr int ROWS = 128 * NT;
   static constexpr int Q_BYTES = ROWS * DP * 2;
   static constexpr int SLOT_BYTES = BN * DP * 2;        // one K or V block
-  static constexpr int FIT = (226 * 1024 - 512 - NT * 1024 - Q_BYTES) / SLOT_BYTES;  // beside the static arrays
-  static constexpr int RING = FIT > 12 ? 12 : FIT;
-  static constexpr int SMEM = 1024 + Q_BYTES + RING * SLOT_BYTES;
+  static constexpr int STAGE_BYTES = 2 * SLOT_BYTES;    // K of a block and V of the one NB before it
+  static constexpr int FIT = (226 * 1024 - 512 - NT * 1024 - Q_BYTES) / STAGE_BYTES;  // beside the static arrays
+  static constexpr int RING = FIT > 6 ? 6 : FIT;
+  static constexpr int SMEM = 1024 + Q_BYTES + RING * STAGE_BYTES;
   static constexpr int O_COL = 0, S_COL = NT * DP;      // tensor memory columns: O, then the score buffers
   static constexpr int TMEM_COLS = 512;
   static constexpr int WARPS = 8 * NT + 1 + NT;         // softmax, producer, issuers
-  static_assert(S_COL + NT * NB * BN <= TMEM_COLS && RING >= NB + 2 && SMEM + NT * 1024 + 512 <= 227 * 1024, "fits");
+  static_assert(S_COL + NT * NB * BN <= TMEM_COLS && RING >= 2 && SMEM + NT * 1024 + 512 <= 227 * 1024, "fits");
 };
 
 struct AttnItem {
@@ -438,10 +439,8 @@ __global__ void __launch_bounds__(AttnCfg<DP, NT>::WARPS * 32, 1)
   const AttnItem it = item_sh;
   const int per_seq = p.T * p.rep;
   const int np = it.pb1 - it.pb0, nblk = np + it.sb1 - it.sb0;
-  // Ring positions, in the order the issuers need them: the first NB K, then V0 K(NB) V1
-  // K(NB + 1) ..., at the end the last NB V.
-  const int lead = min(NB, nblk), late = nblk - lead;
-  auto v_pos = [&](int i) { return lead + i + min(i, late); };
+  // Stage j of the ring holds K(j) and V(j - NB): what the issuers need at one point.
+  const int stages = nblk > 0 ? nblk + NB : 0;
   uint8_t* ring = smem + C::Q_BYTES;
   bool ok = true;
 
@@ -459,25 +458,25 @@ __global__ void __launch_bounds__(AttnCfg<DP, NT>::WARPS * 32, 1)
         }
       }
       int issued = 0;
-      for (int pos = 0; pos < 2 * nblk; ++pos) {
-        const int q = pos - lead;  // from here on V and K take turns
-        const bool is_v = q >= 2 * late || (q >= 0 && (q & 1) == 0);
-        const int i = q < 0 ? pos : q >= 2 * late ? q - late : is_v ? q / 2 : NB + q / 2;
-        const int slot = pos % RING;
-        if (pos >= RING && !mbar_wait(&empty[slot], (pos / RING - 1) & 1, kSiteAttn)) break;
-        mbar_arrive_expect_tx(&full[slot], C::SLOT_BYTES);
-        const bool prefix = i < np;
-        const CUtensorMap* map = prefix ? (is_v ? &tm_pv : &tm_pk) : (is_v ? &tm_v : &tm_k);
-        const int key = (prefix ? it.pb0 + i : it.sb0 + i - np) * BN, who = prefix ? it.g : it.b;
+      for (int j = 0; j < stages; ++j) {
+        const int slot = j % RING;
+        if (j >= RING && !mbar_wait(&empty[slot], (j / RING - 1) & 1, kSiteAttn)) break;
+        mbar_arrive_expect_tx(&full[slot], ((j < nblk) + (j >= NB)) * C::SLOT_BYTES);
+        for (int is_v = 0; is_v < 2; ++is_v) {
+          const int i = is_v ? j - NB : j;
+          if (i < 0 || i >= nblk) continue;
+          const bool prefix = i < np;
+          const CUtensorMap* map = prefix ? (is_v ? &tm_pv : &tm_pk) : (is_v ? &tm_v : &tm_k);
+          const int key = (prefix ? it.pb0 + i : it.sb0 + i - np) * BN, who = prefix ? it.g : it.b;
+          const uint32_t at = smem_u32(ring) + slot * C::STAGE_BYTES + is_v * C::SLOT_BYTES;
 #pragma unroll
-        for (int c = 0; c < DP / 64; ++c)
-          tma_load_4d(smem_u32(ring + slot * C::SLOT_BYTES + c * BN * 128), map, 64 * c, it.kv, key, who,
-                      smem_u32(&full[slot]));
+          for (int c = 0; c < DP / 64; ++c) tma_load_4d(at + c * BN * 128, map, 64 * c, it.kv, key, who, smem_u32(&full[slot]));
+        }
         ++issued;
       }
       // Never leave the CTA with copies still landing in shared memory.
-      for (int pos = issued > RING ? issued - RING : 0; pos < issued; ++pos)
-        mbar_wait(&full[pos % RING], (pos / RING) & 1, kSiteAttn + 1);
+      for (int j = issued > RING ? issued - RING : 0; j < issued; ++j)
+        mbar_wait(&full[j % RING], (j / RING) & 1, kSiteAttn + 1);
       for (int t = 0; p.q_boxes && nblk > 0 && t < NT; ++t) mbar_wait(&q_full[t], 0, kSiteAttn + 1);
     }
   } else if (warp >= kIssuer) {
@@ -488,8 +487,8 @@ __global__ void __launch_bounds__(AttnCfg<DP, NT>::WARPS * 32, 1)
     const int t = warp - kIssuer;
     if (nblk > 0 && lane == 0) {
       const uint64_t q_desc = smem_desc_sw128(smem_u32(smem) + t * (128 * DP * 2));
-      const uint64_t k_desc0 = smem_desc_sw128(smem_u32(ring)), v_desc0 = smem_desc_mn_sw128(smem_u32(ring), BN);
-      constexpr uint32_t kSlotStep = C::SLOT_BYTES >> 4;
+      const uint64_t k_desc0 = smem_desc_sw128(smem_u32(ring)), v_desc0 = smem_desc_mn_sw128(smem_u32(ring) + C::SLOT_BYTES, BN);
+      constexpr uint32_t kStageStep = C::STAGE_BYTES >> 4;
       const uint32_t o_col = tmem + C::O_COL + t * DP, s_col = tmem + C::S_COL + t * NB * BN;
       int slot = 0;
       uint32_t lap = 0;
@@ -497,46 +496,34 @@ __global__ void __launch_bounds__(AttnCfg<DP, NT>::WARPS * 32, 1)
         if (++slot == RING) slot = 0, lap ^= 1;
       };
       auto scores = [&](uint32_t s_at) {  // S = Q K^T
-        const uint64_t k_desc = k_desc0 + (uint32_t)slot * kSlotStep;
+        const uint64_t k_desc = k_desc0 + (uint32_t)slot * kStageStep;
 #pragma unroll
         for (int k = 0; k < DP / 16; ++k)
           mma16_ss(s_at, q_desc + (k / 4) * (128 * 128 / 16) + (k % 4) * 2,
                    k_desc + (k / 4) * (BN * 128 / 16) + (k % 4) * 2, idesc_16<T>(BN, false), k > 0);
       };
       ok = mbar_wait(&q_full[t], 0, kSiteAttn + 2);
-      for (int i = 0; i < lead && ok; ++i) {
-        if (!(ok = mbar_wait(&full[slot], lap, kSiteAttn + 2))) break;
-        tc_fence_after();
-        scores(s_col + i * BN);
-        mma_commit(&step[t][i]);
-        mma_commit(&empty[slot]);
-        next();
-      }
       int buffer = 0;
       uint32_t turn = 0;  // p_ready's phase
-      for (int i = 0; i < nblk && ok; ++i) {
-        const uint64_t v_desc = v_desc0 + (uint32_t)slot * kSlotStep;
+      for (int i = -NB; i < nblk && ok; ++i) {
+        // O += P(i) V(i), then S(i + NB) = Q K^T over the p just taken.
         const uint32_t s_at = s_col + buffer * BN;
-        ok = mbar_wait(&full[slot], lap, kSiteAttn + 2) && mbar_wait(&p_ready[t][buffer], turn, kSiteAttn + 3);
+        ok = mbar_wait(&full[slot], lap, kSiteAttn + 2) &&
+             (i < 0 || mbar_wait(&p_ready[t][buffer], turn, kSiteAttn + 3));
         if (!ok) break;
         tc_fence_after();
+        if (i >= 0) {
+          const uint64_t v_desc = v_desc0 + (uint32_t)slot * kStageStep;
 #pragma unroll
-        for (int k = 0; k < BN / 16; ++k)  // O += P V; each half of the keys has its p over its own scores
-          mma16_ts(o_col, s_at + (k / (BN / 32)) * (BN / 2) + (k % (BN / 32)) * 8, v_desc + k * (2048 / 16),
-                   idesc_16<T>(DP, true), i > 0 || k > 0);
+          for (int k = 0; k < BN / 16; ++k)  // each half of the keys has its p over its own scores
+            mma16_ts(o_col, s_at + (k / (BN / 32)) * (BN / 2) + (k % (BN / 32)) * 8, v_desc + k * (2048 / 16),
+                     idesc_16<T>(DP, true), i > 0 || k > 0);
+        }
+        if (i + NB < nblk) scores(s_at);
+        mma_commit(&step[t][buffer]);
         mma_commit(&empty[slot]);
         next();
-        if (i + NB < nblk) {
-          if (!(ok = mbar_wait(&full[slot], lap, kSiteAttn + 2))) break;
-          tc_fence_after();
-          scores(s_at);  // over the p that O just took
-          mma_commit(&step[t][buffer]);
-          mma_commit(&empty[slot]);
-          next();
-        } else {
-          mma_commit(&step[t][buffer]);
-        }
-        if (++buffer == NB) buffer = 0, turn ^= 1;
+        if (++buffer == NB) buffer = 0, turn ^= i >= 0;
       }
       if (ok) {
         const int last = nblk - 1 + NB;
@@ -594,6 +581,8 @@ __global__ void __launch_bounds__(AttnCfg<DP, NT>::WARPS * 32, 1)
     int buffer = 0;
     uint32_t turn = 0;
     for (int i = 0; i < nblk; ++i) {
+      ok = ok && mbar_wait(&step[t][buffer], turn, kSiteAttn + 6);
+      ok = __all_sync(0xffffffffu, ok);
       const bool masked = i == mask_prefix || i >= own_mask;
       int end = BN;  // keys of this half that the row sees
       if (masked) {
@@ -601,12 +590,14 @@ __global__ void __launch_bounds__(AttnCfg<DP, NT>::WARPS * 32, 1)
         const int key = (prefix ? it.pb0 + i : it.sb0 + i - np) * BN;
         end = (prefix ? it.plen : own_end) - key - half * HALF;
         // Cache rows past the length may hold anything, and p = 0 would not hide a NaN.
-        // (Each tile clears them before its own product; the second time changes nothing.)
+        // (Each tile clears them before its own product; the second time changes nothing.
+        // The step above says that this stage's last use is over, so that its next phase is
+        // the one waited for.)
         const int filled = (prefix ? it.plen : it.slen) - key;
         if (filled < BN && key + filled < (prefix ? p.P : p.S)) {
-          const int pos = v_pos(i);
-          ok = ok && mbar_wait(&full[pos % RING], (pos / RING) & 1, kSiteAttn + 5);
-          uint8_t* v = ring + (pos % RING) * C::SLOT_BYTES;
+          const int j = i + NB;
+          ok = ok && mbar_wait(&full[j % RING], (j / RING) & 1, kSiteAttn + 5);
+          uint8_t* v = ring + (j % RING) * C::STAGE_BYTES + C::SLOT_BYTES;
           const int gone = BN - filled;
           for (int c = threadIdx.x & 255; c < gone * (DP / 8); c += 256) {
             const int rr = filled + c % gone, col = c / gone;
@@ -615,8 +606,6 @@ __global__ void __launch_bounds__(AttnCfg<DP, NT>::WARPS * 32, 1)
           fence_proxy_async_smem();
         }
       }
-      ok = ok && mbar_wait(&step[t][buffer], turn, kSiteAttn + 6);
-      ok = __all_sync(0xffffffffu, ok);
       const uint32_t s_addr = s_addr0 + buffer * BN;
       uint32_t x[32], pk[16];
       if (!idle) {
@@ -736,7 +725,7 @@ __global__ void __launch_bounds__(AttnCfg<DP, NT>::WARPS * 32, 1)
         }
         __syncwarp();
         const int per = p.splits == 1 ? 8 : 4;  // columns of a piece
-#pragma unroll 8
+#pragma unroll 4
         for (int c = lane; c < 32 * CH; c += 32) {
           const int r = c / CH, j = c % CH;
           const int at = __shfl_sync(0xffffffffu, live ? row : -1, r), d = col + j * per;
