@@ -250,19 +250,6 @@ __device__ __forceinline__ float exp2_approx(float x) {
   return y;
 }
 
-template <typename T>
-__device__ __forceinline__ uint32_t pack16(float a, float b);
-template <>
-__device__ __forceinline__ uint32_t pack16<__nv_bfloat16>(float a, float b) {
-  const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
-  return *reinterpret_cast<const uint32_t*>(&h);
-}
-template <>
-__device__ __forceinline__ uint32_t pack16<__half>(float a, float b) {
-  const __half2 h = __floats2half2_rn(a, b);
-  return *reinterpret_cast<const uint32_t*>(&h);
-}
-
 // DP: the head size rounded up to 64, 128 or 256 (the rest of a row is zeros).
 // NT: row tiles of 128 per CTA.
 template <int DP, int NT>

@@ -83,6 +83,30 @@ def test_matches_the_formula(rows, width, dtype):
     run_and_check(x, residual, m, scale=0.7)
 
 
+# Enough rows for the kernel that streams them (16 per SM).
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
+@pytest.mark.parametrize("rows,width", [(2400, 520), (2501, 1000), (2600, 2048), (2387, 2056), (3001, 4096),
+                                        (2400, 8192), (2400, 264), (5000, 776)])
+def test_many_rows(rows, width, dtype):
+    x, residual, m = operands(rows, width, dtype, rows + width)
+    run_and_check(x, residual, m, scale=0.7)
+
+
+@pytest.mark.parametrize("width", [640, 1536, 4096])
+@pytest.mark.parametrize("post,gate,shift,groups", [(None, "group", "group", 1250), ("group", None, None, 5),
+                                                    ("width", "group", "group", 2500), (None, None, "group", 100)])
+def test_many_rows_with_modulations(width, post, gate, shift, groups):
+    from actune_b200 import ops
+    x, residual, m = operands(2500, width, torch.bfloat16, groups, post=post, gate=gate, shift=shift, pre="group",
+                              groups=groups)
+    wide = torch.cat([x, residual], 1)
+    h, _ = run_and_check(wide[:, :width], wide[:, width:], m, gemma=True)
+    got = ops.gated_norm(wide[:, :width], wide[:, width:], m["pre_weight"], post_weight=m["post_weight"],
+                         gate=m["gate"], shift=m["shift"], gemma=True, quant_bits=4)
+    want, scales = ops.quantize_group64(h, 4)
+    assert torch.equal(got[0], h) and torch.equal(got[2], want) and torch.equal(got[3], scales)
+
+
 @pytest.mark.parametrize("gemma", [False, True])
 @pytest.mark.parametrize("post", [None, "width", "group"])
 @pytest.mark.parametrize("gate", [None, "width", "group"])
