@@ -1,7 +1,7 @@
 // Low-rank adapters of many requests beside a shared projection (sm_100a):
 //   out[m] = y[m] + scale[s] * up[s] (down[s] x[m]),   s = slots[m].
 //
-// plan    rows sorted by adapter into tiles of 16, 32 or 64 rows with one adapter each.
+// plan    rows sorted by adapter into tiles of 4, 16, 32 or 128 rows with one adapter each.
 // shrink  v = down x for a tile and a slice of K; the slices' fp32 sums go to the
 //         workspace, so that few rows still occupy the machine, in a fixed order.
 // expand  out = y + scale * up v for a tile and a range of columns.
@@ -20,6 +20,7 @@ namespace {
 
 constexpr int kMaxSlots = 8191;
 constexpr int kMaxRank = 128;
+constexpr int kFewRows = 4;
 constexpr int kHeader = 4;  // plan: tile count, then three padding words
 
 // Tiles of `tile` rows that M rows of S adapters (and of none) can make at most.
@@ -98,7 +99,10 @@ struct AdapterParams {
   const float* scale;
   const int32_t* plan;
   void* out;
-  float* v;  // [slices, M, RP] partial sums of down x, rows in plan order
+  float* v;       // [slices, M, RP] partial sums of down x, rows in plan order; or, for tiles of 128,
+  void* split;    // [2, M, RP]: down x as hi and lo parts, and
+  float* factor;  // [M]: what a row's product with `up` is multiplied by
+  int boxes;      // y and out have tensor maps
   int64_t x_stride, y_stride, out_stride;
   int M, N, K, S, R, tiles_cap;
   int slices, k_slice;  // K elements per slice, a multiple of 128
@@ -146,19 +150,46 @@ __device__ __forceinline__ void load_run(uint32_t (&r)[COUNT / 2], const T* row,
   }
 }
 
-// v[slice, position, 0 .. RP) for one tile and one slice of K.  WM warps side by side
-// along the rows (16 each) and 4 / WM along K; a warp's K steps are 32 elements: lane
-// (g, t) holds elements 8t .. 8t + 7 of rows g and g + 8 of x and of row g of each
-// 8-row block of down, two MMAs per block.  Nothing is shared between warps until
-// their sums are added in shared memory.
-template <typename T, int WM, int RP, bool VEC>
-__global__ void __launch_bounds__(128) adapter_shrink_kernel(const AdapterParams p) {
-  constexpr int WK = 4 / WM, NT = RP / 8;
-  __shared__ float part[WK > 1 ? (WK - 1) * WM * 16 * RP : 1];
+// fp16 has 5 exponent bits: the power of two that brings a row's largest |v| into [1, 2)
+// (`down`), and what undoes it (returned).  1 for rows of zeros and of infinities.
+__device__ __forceinline__ float fp16_room(float top, float& down) {
+  const bool some = top > 0.f && top < __int_as_float(0x7f800000);
+  const int e = some ? max(ilogbf(top), -100) : 0;
+  down = scalbnf(1.f, -e);
+  return scalbnf(1.f, e);
+}
+
+// v = hi + lo in T (lo the rounding error of hi, itself rounded).
+template <typename T>
+__device__ __forceinline__ void split2(float a, float b, uint32_t& hi, uint32_t& lo) {
+  const T ah = narrow<T>(a), bh = narrow<T>(b);
+  const float al = a - widen<T>(ah), bl = b - widen<T>(bh);
+  // An infinity has no remainder (inf - inf would make a NaN of it).
+  const T parts[4] = {ah, bh, narrow<T>(isfinite(a) ? al : 0.f), narrow<T>(isfinite(b) ? bl : 0.f)};
+  hi = *reinterpret_cast<const uint32_t*>(&parts[0]);
+  lo = *reinterpret_cast<const uint32_t*>(&parts[2]);
+}
+
+// v = down x for WM * 16 rows of a tile.  WM warps side by side along the rows (16 each)
+// and WK along K; a warp's K steps are 32 elements: lane (g, t) holds elements 8t .. 8t + 7
+// of rows g and g + 8 of x and of row g of each 8-row block of down, two MMAs per block.
+// Nothing is shared between warps until their sums are added in shared memory.
+//
+// SPLIT: a quarter of a 128-row tile and all of K, 8 warps; the sums are complete, and go
+// out as the two 16-bit parts that the next kernel takes.  Else a tile and one slice of K;
+// the slice's sums go out in fp32.
+constexpr int shrink_warps(int wm, bool split) { return split || wm > 4 ? 8 : 4; }
+constexpr int shrink_shared(int wm, int rp, bool split) { return (shrink_warps(wm, split) / wm - 1) * wm * 16 * rp * 4; }
+
+template <typename T, int WM, int RP, bool VEC, bool SPLIT>
+__global__ void __launch_bounds__(32 * shrink_warps(WM, SPLIT)) adapter_shrink_kernel(const AdapterParams p) {
+  constexpr int WK = shrink_warps(WM, SPLIT) / WM, NT = RP / 8;
+  extern __shared__ float part[];  // [WK - 1, WM, 16 * RP]
   griddep_enter();
   if ((int)blockIdx.x >= p.plan[0]) return;
-  const int4 tile = plan_tiles(p.plan)[blockIdx.x];
-  if (tile.x < 0) return;
+  int4 tile = plan_tiles(p.plan)[blockIdx.x];
+  if constexpr (SPLIT) tile.y += blockIdx.y * (WM * 16), tile.z -= blockIdx.y * (WM * 16);
+  if (tile.x < 0 || tile.z <= 0) return;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int g = lane >> 2, t = lane & 3;
   const int wm = warp % WM, wk = warp / WM;
@@ -170,10 +201,11 @@ __global__ void __launch_bounds__(128) adapter_shrink_kernel(const AdapterParams
     rows[h] = i < tile.z ? reinterpret_cast<const T*>(p.x) + order[i] * p.x_stride : nullptr;
   }
   const T* down = reinterpret_cast<const T*>(p.down) + (int64_t)tile.x * p.R * p.K;
-  const int k0 = blockIdx.y * p.k_slice, k1 = min(p.K, k0 + p.k_slice);
+  const int k0 = SPLIT ? 0 : blockIdx.y * p.k_slice, k1 = SPLIT ? p.K : min(p.K, k0 + p.k_slice);
   float acc[NT][4] = {};
   if (wm * 16 < tile.z) {
-#pragma unroll 2
+    constexpr int UNROLL = RP <= 64 ? 4 : 2;  // steps whose loads go out together
+#pragma unroll UNROLL
     for (int k = k0 + wk * 32; k < k1; k += WK * 32) {
       const int e = k + 8 * t;
       uint32_t xa[2][4], db[NT][4];
@@ -211,28 +243,115 @@ __global__ void __launch_bounds__(128) adapter_shrink_kernel(const AdapterParams
 #pragma unroll
   for (int h = 0; h < 2; ++h) {
     const int i = wm * 16 + g + 8 * h;
-    if (i >= tile.z) continue;
-    float* dst = p.v + ((int64_t)blockIdx.y * p.M + tile.y + i) * RP + 2 * t;
+    if constexpr (SPLIT) {
+      float down_by = 1.f, factor = p.scale[tile.x];
+      if constexpr (std::is_same<T, __half>::value) {
+        float top = 0.f;
 #pragma unroll
-    for (int j = 0; j < NT; ++j) *reinterpret_cast<float2*>(dst + j * 8) = make_float2(acc[j][2 * h], acc[j][2 * h + 1]);
+        for (int j = 0; j < NT; ++j) top = fmaxf(top, fmaxf(fabsf(acc[j][2 * h]), fabsf(acc[j][2 * h + 1])));
+        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+        factor *= fp16_room(top, down_by);
+      }
+      if (i >= tile.z) continue;
+      if (t == 0) p.factor[tile.y + i] = factor;
+      T* dst = reinterpret_cast<T*>(p.split) + (int64_t)(tile.y + i) * RP + 2 * t;
+#pragma unroll
+      for (int j = 0; j < NT; ++j) {
+        uint32_t hi, lo;
+        split2<T>(acc[j][2 * h] * down_by, acc[j][2 * h + 1] * down_by, hi, lo);
+        *reinterpret_cast<uint32_t*>(dst + j * 8) = hi;
+        *reinterpret_cast<uint32_t*>(dst + (int64_t)p.M * RP + j * 8) = lo;
+      }
+    } else {
+      if (i >= tile.z) continue;
+      float* dst = p.v + ((int64_t)blockIdx.y * p.M + tile.y + i) * RP + 2 * t;
+#pragma unroll
+      for (int j = 0; j < NT; ++j) *reinterpret_cast<float2*>(dst + j * 8) = make_float2(acc[j][2 * h], acc[j][2 * h + 1]);
+    }
   }
 }
 
-// v = hi + lo in T (lo the rounding error of hi, itself rounded).
-template <typename T>
-__device__ __forceinline__ void split2(float a, float b, uint32_t& hi, uint32_t& lo) {
-  const T ah = narrow<T>(a), bh = narrow<T>(b);
-  const float al = a - widen<T>(ah), bl = b - widen<T>(bh);
-  // An infinity has no remainder (inf - inf would make a NaN of it).
-  const T parts[4] = {ah, bh, narrow<T>(isfinite(a) ? al : 0.f), narrow<T>(isfinite(b) ? bl : 0.f)};
-  hi = *reinterpret_cast<const uint32_t*>(&parts[0]);
-  lo = *reinterpret_cast<const uint32_t*>(&parts[2]);
+// out = y + scale * up v for tiles of kFewRows rows, the single-token case: a thread has
+// pairs of columns, reads their rows of `up` 16 bytes at a time (requested before v is
+// there, which nothing but the sum over the slices separates from the kernel's start) and
+// adds up the products in fp32.  32 requests of one token, 4096 -> 22016, rank 16: 17 us
+// with the matrix instructions of the other form, whose loads depend on one another.
+template <typename T, int RP>
+__global__ void __launch_bounds__(128) adapter_expand_few_kernel(const AdapterParams p) {
+  constexpr int PAIRS = RP == 16 ? 2 : 1, PIECES = RP / 8;
+  __shared__ float v[kFewRows * RP];
+  griddep_enter();
+  if ((int)blockIdx.y >= p.plan[0]) return;
+  const int4 tile = plan_tiles(p.plan)[blockIdx.y];
+  if (tile.x < 0 && p.out == p.y) return;
+  const T* up = reinterpret_cast<const T*>(p.up) + (int64_t)max(tile.x, 0) * p.N * p.R;
+  const int32_t* order = plan_rows(p) + tile.y;
+  const int begin = blockIdx.x * p.col_steps * 256, end = min(p.N, begin + p.col_steps * 256);
+  const int pieces = tile.x >= 0 ? p.R / 8 : 0;
+  for (int n0 = begin; n0 < end; n0 += 256 * PAIRS) {
+    Raw8<T> w[PAIRS][2][PIECES];
+    uint32_t yv[PAIRS][kFewRows];
+#pragma unroll
+    for (int c = 0; c < PAIRS; ++c) {
+      const int n = n0 + 2 * (threadIdx.x + 128 * c);
+      if (n >= end) continue;
+#pragma unroll
+      for (int e = 0; e < 2; ++e)
+#pragma unroll
+        for (int k = 0; k < PIECES; ++k)
+          if (k < pieces) w[c][e][k].load(up + (int64_t)(n + e) * p.R + 8 * k);
+#pragma unroll
+      for (int r = 0; r < kFewRows; ++r)
+        if (r < tile.z) yv[c][r] = *reinterpret_cast<const uint32_t*>(reinterpret_cast<const T*>(p.y) + order[r] * p.y_stride + n);
+    }
+    if (n0 == begin) {
+      for (int i = threadIdx.x; i < tile.z * RP; i += 128) {
+        float a = 0.f;
+        for (int s = 0; tile.x >= 0 && s < p.slices; s += 8) {  // eight loads at a time, added in order
+          float part[8];
+#pragma unroll
+          for (int u = 0; u < 8; ++u)
+            part[u] = s + u < p.slices ? p.v[((int64_t)(s + u) * p.M + tile.y) * RP + i] : 0.f;
+#pragma unroll
+          for (int u = 0; u < 8; ++u) a += part[u];
+        }
+        v[i] = tile.x >= 0 ? a * p.scale[tile.x] : 0.f;
+      }
+      __syncthreads();
+    }
+#pragma unroll
+    for (int c = 0; c < PAIRS; ++c) {
+      const int n = n0 + 2 * (threadIdx.x + 128 * c);
+      if (n >= end) continue;
+#pragma unroll
+      for (int r = 0; r < kFewRows; ++r) {
+        if (r >= tile.z) break;
+        float2 a = make_float2(0.f, 0.f);
+#pragma unroll
+        for (int k = 0; k < PIECES; ++k) {
+          if (k >= pieces) break;
+          float f[8], g[8];
+          w[c][0][k].get(f);
+          w[c][1][k].get(g);
+#pragma unroll
+          for (int i = 0; i < 8; ++i) {
+            const float x = v[r * RP + 8 * k + i];
+            a.x = fmaf(x, f[i], a.x), a.y = fmaf(x, g[i], a.y);
+          }
+        }
+        const float2 y = unpack16<T>(yv[c][r]);
+        *reinterpret_cast<uint32_t*>(reinterpret_cast<T*>(p.out) + order[r] * p.out_stride + n) =
+            pieces > 0 ? pack16<T>(y.x + a.x, y.y + a.y) : yv[c][r];
+      }
+    }
+  }
 }
 
 // out = y + scale * up v.  A warp keeps the split v of MW * 16 rows in registers and
 // walks col_steps steps of 64 columns; the columns of a step are dealt so that lane
-// (g, t) ends up with columns 16t .. 16t + 15 of rows g and g + 8: 32 contiguous bytes
-// of y and out.
+// (g, t) ends up with columns 8t .. 8t + 7 and 32 + 8t .. 32 + 8t + 7 of rows g and g + 8:
+// a quad's 16-byte pieces of y and out lie side by side.
 template <typename T, int WM, int MW, int RP, bool VEC>
 __global__ void __launch_bounds__(128) adapter_expand_kernel(const AdapterParams p) {
   constexpr int WN = 4 / WM, KS = RP / 16;
@@ -262,28 +381,32 @@ __global__ void __launch_bounds__(128) adapter_expand_kernel(const AdapterParams
       for (int k = 0; k < KS; ++k) v[k] = make_float4(0.f, 0.f, 0.f, 0.f);
       if (i < tile.z && tile.x >= 0) {
         const float* src = p.v + (int64_t)(tile.y + i) * RP + 4 * t;
-        for (int s = 0; s < p.slices; ++s, src += (int64_t)p.M * RP)
+        constexpr int U = KS <= 2 ? 4 : 1;  // slices whose loads go out together
+        for (int s = 0; s < p.slices; s += U, src += U * (int64_t)p.M * RP) {
+          float4 a[U][KS];
 #pragma unroll
-          for (int k = 0; k < KS; ++k) {
-            const float4 a = *reinterpret_cast<const float4*>(src + 16 * k);
-            v[k].x += a.x, v[k].y += a.y, v[k].z += a.z, v[k].w += a.w;
-          }
+          for (int u = 0; u < U; ++u)
+#pragma unroll
+            for (int k = 0; k < KS; ++k)
+              a[u][k] = s + u < p.slices ? *reinterpret_cast<const float4*>(src + u * (int64_t)p.M * RP + 16 * k)
+                                         : make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+          for (int u = 0; u < U; ++u)
+#pragma unroll
+            for (int k = 0; k < KS; ++k) v[k].x += a[u][k].x, v[k].y += a[u][k].y, v[k].z += a[u][k].z, v[k].w += a[u][k].w;
+        }
       }
       factor[m][h] = scale;
-      if constexpr (sizeof(T) == 2 && !std::is_same<T, __nv_bfloat16>::value) {
-        // fp16 has 5 exponent bits: bring the row's largest |v| into [1, 2) first.
+      if constexpr (std::is_same<T, __half>::value) {
 #pragma unroll
         for (int k = 0; k < KS; ++k)
           top = fmaxf(fmaxf(top, fmaxf(fabsf(v[k].x), fabsf(v[k].y))), fmaxf(fabsf(v[k].z), fabsf(v[k].w)));
         top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
         top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
-        if (top > 0.f && top < __int_as_float(0x7f800000)) {
-          const int e = max(ilogbf(top), -100);
-          const float down = scalbnf(1.f, -e);
+        float down;
+        factor[m][h] = scale * fp16_room(top, down);
 #pragma unroll
-          for (int k = 0; k < KS; ++k) v[k].x *= down, v[k].y *= down, v[k].z *= down, v[k].w *= down;
-          factor[m][h] = scale * scalbnf(1.f, e);
-        }
+        for (int k = 0; k < KS; ++k) v[k].x *= down, v[k].y *= down, v[k].z *= down, v[k].w *= down;
       }
 #pragma unroll
       for (int k = 0; k < KS; ++k) {
@@ -297,7 +420,7 @@ __global__ void __launch_bounds__(128) adapter_expand_kernel(const AdapterParams
   for (int step = 0; step < p.col_steps; ++step) {
     const int n0 = (blockIdx.x * p.col_steps + step) * span + wn * 64;
     if (n0 >= p.N) break;
-    const int n = n0 + 16 * t;
+    const int n = n0 + 8 * t;
     uint32_t yv[MW][2][2][4];
 #pragma unroll
     for (int m = 0; m < MW; ++m)
@@ -305,7 +428,7 @@ __global__ void __launch_bounds__(128) adapter_expand_kernel(const AdapterParams
       for (int h = 0; h < 2; ++h)
 #pragma unroll
         for (int c = 0; c < 2; ++c)
-          load_run<T, VEC, 8>(yv[m][h][c], reinterpret_cast<const T*>(p.y) + row[m][h] * p.y_stride, n + 8 * c,
+          load_run<T, VEC, 8>(yv[m][h][c], reinterpret_cast<const T*>(p.y) + row[m][h] * p.y_stride, n + 32 * c,
                               row[m][h] >= 0 ? p.N : 0);
     float acc[MW][8][4] = {};
     if (tile.x >= 0) {
@@ -313,7 +436,7 @@ __global__ void __launch_bounds__(128) adapter_expand_kernel(const AdapterParams
       for (int k = 0; k < KS; ++k) {
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
-          const int col = n0 + 16 * (g >> 1) + 2 * j + (g & 1);
+          const int col = n0 + 32 * (j >> 2) + 8 * (g >> 1) + 2 * (j & 3) + (g & 1);
           uint32_t b[2];
           load_run<T, VEC, 4>(b, up + (int64_t)col * p.R, 16 * k + 4 * t, col < p.N ? p.R : 0);
 #pragma unroll
@@ -340,15 +463,257 @@ __global__ void __launch_bounds__(128) adapter_expand_kernel(const AdapterParams
             o[i] = tile.x >= 0 ? narrow<T>(fmaf(factor[m][h], d, widen<T>(yt[i]))) : yt[i];
           }
           if constexpr (VEC) {
-            if (n + 8 * c < p.N) *reinterpret_cast<uint4*>(dst + n + 8 * c) = *reinterpret_cast<const uint4*>(o);
+            if (n + 32 * c < p.N) *reinterpret_cast<uint4*>(dst + n + 32 * c) = *reinterpret_cast<const uint4*>(o);
           } else {
 #pragma unroll
             for (int i = 0; i < 8; ++i)
-              if (n + 8 * c + i < p.N) dst[n + 8 * c + i] = o[i];
+              if (n + 32 * c + i < p.N) dst[n + 32 * c + i] = o[i];
           }
         }
       }
   }
+}
+
+// The same for tiles of 128 rows on the tcgen05 tensor cores: D[128 rows, 128 columns] =
+// V up^T, with V = hi + lo kept in shared memory as two K-major operands and the rows of
+// `up` as the other, brought by TMA, two products into one accumulator.
+//
+// With the products out of the way the kernel is what its traffic makes it: y in, out out.
+// Both go through a ring of stages in shared memory, several steps ahead, where the
+// accumulator's thread of a row (as tensor memory has it) adds its columns in place.  32
+// rows that follow one another, as a request's do, come and go as boxes by TMA; others
+// through 16-byte asynchronous copies and coalesced stores.  4864 x 32768, rank 64, y in
+// and out alone: 167 us by the warps' own loads and stores, 294 us by a bulk copy of 256
+// bytes per row (about 30 cycles each), 99 us for a plain copy of the same bytes.
+// 8 epilogue warps, four a step (32 rows each), alternating; a producer warp for y, one for
+// V and up, an MMA issuer; two accumulators.
+template <int RP>
+struct ExpandCfg {
+  static constexpr int SUB = RP > 64 ? 2 : 1;          // 64-wide K tiles of 128-byte rows
+  static constexpr int TILE_BYTES = SUB * 128 * 128;   // 128 rows
+  static constexpr int RING = 2;
+  static constexpr int Y_BYTES = 2 * 128 * 128;        // 128 rows of y in two 64-column tiles, swizzled
+  static constexpr int FIT = (226 * 1024 - 512 - (2 + RING) * TILE_BYTES) / Y_BYTES;
+  static constexpr int Y_RING = FIT > 4 ? 4 : FIT;
+  static constexpr int SMEM = 1024 + (2 + RING) * TILE_BYTES + Y_RING * Y_BYTES;
+  static constexpr int THREADS = 32 * 11;
+  static_assert(Y_RING >= 3, "a step under way for each half of the epilogue and one behind them");
+};
+constexpr int kSiteAdapter = 310;
+
+template <typename T, int RP>
+__global__ void __launch_bounds__(ExpandCfg<RP>::THREADS, 1)
+    adapter_expand128_kernel(const __grid_constant__ CUtensorMap tm_up, const __grid_constant__ CUtensorMap tm_v,
+                             const __grid_constant__ CUtensorMap tm_y, const __grid_constant__ CUtensorMap tm_out,
+                             const AdapterParams p) {
+  using C = ExpandCfg<RP>;
+  constexpr int RING = C::RING, Y_RING = C::Y_RING;
+  extern __shared__ uint8_t smem_raw[];
+  __shared__ __align__(8) uint64_t full[RING], empty[RING], d_full[2], d_empty[2], y_full[Y_RING], y_empty[Y_RING];
+  __shared__ __align__(8) uint64_t v_ready, drained;
+  __shared__ uint32_t tmem_holder;
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  uint8_t* ring = smem + 2 * C::TILE_BYTES;
+  uint8_t* y_ring = ring + RING * C::TILE_BYTES;
+  const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
+  constexpr int kYProducer = 8, kProducer = 9, kIssuer = 10;
+  if (warp == kIssuer) {
+    tmem_alloc(&tmem_holder, 256);
+    tmem_relinquish();
+  }
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < RING; ++i) {
+      mbar_init(&full[i], 1);
+      mbar_init(&empty[i], 1);
+    }
+    for (int i = 0; i < Y_RING; ++i) {
+      mbar_init(&y_full[i], 33);  // the producer's lanes, and its box bytes
+      mbar_init(&y_empty[i], 4);
+    }
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(&d_full[i], 1);
+      mbar_init(&d_empty[i], 4);
+    }
+    mbar_init(&v_ready, 1);
+    mbar_init(&drained, 1);
+    fence_barrier_init();
+    prefetch_tensormap(&tm_up);
+    prefetch_tensormap(&tm_v);
+    prefetch_tensormap(&tm_y);
+    prefetch_tensormap(&tm_out);
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  griddep_enter();
+  const uint32_t tmem = tmem_holder;
+  const bool have = (int)blockIdx.y < p.plan[0];
+  const int4 tile = have ? plan_tiles(p.plan)[blockIdx.y] : make_int4(-1, 0, 0, 0);
+  const bool adapted = tile.x >= 0;
+  const int begin = blockIdx.x * p.col_steps * 128, end = min(p.N, begin + p.col_steps * 128);
+  const int steps = have && !(tile.x < 0 && p.out == p.y) ? (end - begin + 127) / 128 : 0;
+  const int32_t* order = plan_rows(p) + tile.y;
+  bool ok = true;
+  // 32 rows of the tile (quarter q) as a box: all there, one after the other.
+  const auto boxed = [&](int q) {
+    return p.boxes && 32 * q + 32 <= tile.z && order[32 * q + 31] - order[32 * q] == 31;
+  };
+  if (warp == kYProducer) {
+    int at[4];  // a quarter's first row if it is a box; else -1
+    const T* rows[4];
+    int boxes = 0;
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+      at[q] = steps > 0 && boxed(q) ? order[32 * q] : -1;
+      boxes += at[q] >= 0;
+      const int r = 32 * q + lane;
+      rows[q] = steps > 0 && at[q] < 0 && r < tile.z ? reinterpret_cast<const T*>(p.y) + order[r] * p.y_stride : nullptr;
+    }
+    int issued = 0;
+    for (int i = 0; i < steps; ++i) {
+      const int slot = i % Y_RING, col = begin + 128 * i;
+      ok = i < Y_RING || mbar_wait(&y_empty[slot], (i / Y_RING - 1) & 1, kSiteAdapter + 7);
+      if (!(ok = __all_sync(0xffffffffu, ok))) break;
+      uint8_t* stage = y_ring + slot * C::Y_BYTES;
+      if (lane == 0) {
+        mbar_arrive_expect_tx(&y_full[slot], boxes * 2 * 32 * 128);
+#pragma unroll
+        for (int q = 0; q < 4; ++q)
+          if (at[q] >= 0)
+            for (int c = 0; c < 2; ++c)
+              tma_load_2d(stage + c * (128 * 128) + q * (32 * 128), &tm_y, col + 64 * c, at[q], &y_full[slot]);
+      }
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        if (at[q] >= 0 || 32 * q >= tile.z) continue;
+        for (int r = 0; r < min(32, tile.z - 32 * q); r += 2) {  // 16 lanes a row
+          const int mine = r + (lane >> 4), piece = lane & 15;
+          const T* src = reinterpret_cast<const T*>(__shfl_sync(0xffffffffu, (unsigned long long)rows[q], mine));
+          const bool there = src != nullptr && col + 8 * piece < end;
+          copy16_or_zero(smem_u32(stage) + (piece >> 3) * (128 * 128) + (32 * q + mine) * 128 + (((piece & 7) ^ (mine & 7)) << 4),
+                         there ? src + col + 8 * piece : reinterpret_cast<const T*>(p.y), there);
+        }
+      }
+      copy16_arrive(&y_full[slot]);
+      ++issued;
+    }
+    // Never leave the CTA with copies still landing in shared memory.
+    for (int i = issued > Y_RING ? issued - Y_RING : 0; i < issued; ++i)
+      mbar_wait(&y_full[i % Y_RING], (i / Y_RING) & 1, kSiteAdapter + 8);
+  } else if (warp == kProducer) {
+    if (lane == 0 && adapted && steps > 0) {
+      // Rows behind the tile's are another's, and nothing reads their products.
+      mbar_arrive_expect_tx(&v_ready, 2 * C::TILE_BYTES);
+      for (int part = 0; part < 2; ++part)
+        for (int c = 0; c < C::SUB; ++c)
+          tma_load_3d(smem + part * C::TILE_BYTES + c * (128 * 128), &tm_v, 64 * c, tile.y, part, &v_ready);
+      int issued = 0;
+      for (int i = 0; i < steps; ++i) {
+        const int slot = i % RING;
+        if (i >= RING && !mbar_wait(&empty[slot], (i / RING - 1) & 1, kSiteAdapter)) break;
+        mbar_arrive_expect_tx(&full[slot], C::TILE_BYTES);
+        for (int c = 0; c < C::SUB; ++c)
+          tma_load_3d(ring + slot * C::TILE_BYTES + c * (128 * 128), &tm_up, 64 * c, begin + 128 * i, tile.x, &full[slot]);
+        ++issued;
+      }
+      for (int i = issued > RING ? issued - RING : 0; i < issued; ++i)
+        mbar_wait(&full[i % RING], (i / RING) & 1, kSiteAdapter + 1);
+      mbar_wait(&v_ready, 0, kSiteAdapter + 1);
+    }
+  } else if (warp == kIssuer) {
+    if (lane == 0 && adapted && steps > 0) {
+      const uint64_t hi = smem_desc_sw128(smem_u32(smem)), lo = smem_desc_sw128(smem_u32(smem) + C::TILE_BYTES);
+      const uint64_t up0 = smem_desc_sw128(smem_u32(ring));
+      int slot = 0;
+      uint32_t lap = 0;
+      ok = mbar_wait(&v_ready, 0, kSiteAdapter + 2);
+      for (int i = 0; i < steps && ok; ++i) {
+        ok = mbar_wait(&full[slot], lap, kSiteAdapter + 3) &&
+             (i < 2 || mbar_wait(&d_empty[i & 1], ((i >> 1) - 1) & 1, kSiteAdapter + 4));
+        if (!ok) break;
+        tc_fence_after();
+        const uint64_t up = up0 + (uint32_t)slot * (C::TILE_BYTES >> 4);
+#pragma unroll
+        for (int k = 0; k < RP / 16; ++k) {
+          const uint32_t at = (k / 4) * (128 * 128 / 16) + (k % 4) * 2;
+          mma16_ss(tmem + (i & 1) * 128, hi + at, up + at, idesc_16<T>(128, false), k > 0);
+        }
+#pragma unroll
+        for (int k = 0; k < RP / 16; ++k) {
+          const uint32_t at = (k / 4) * (128 * 128 / 16) + (k % 4) * 2;
+          mma16_ss(tmem + (i & 1) * 128, lo + at, up + at, idesc_16<T>(128, false), 1);
+        }
+        mma_commit(&empty[slot]);
+        mma_commit(&d_full[i & 1]);
+        if (++slot == RING) slot = 0, lap ^= 1;
+      }
+      mma_commit(&drained);
+      mbar_wait(&drained, 0, kSiteAdapter + 5);  // nothing in flight reads shared memory after this
+    }
+  } else {
+    const int turn = warp >> 2, quarter = warp & 3, row = quarter * 32 + lane;
+    const bool idle = quarter * 32 >= tile.z, box = steps > 0 && boxed(quarter);
+    const float factor = adapted && row < tile.z ? p.factor[tile.y + row] : 0.f;
+    const int mine = steps > 0 && row < tile.z ? order[row] : -1;
+    int sent = -1;  // the slot whose box may still be on its way out
+    for (int i = turn; i < steps; i += 2) {
+      const int slot = i % Y_RING, col = begin + 128 * i;
+      ok = ok && mbar_wait(&y_full[slot], (i / Y_RING) & 1, kSiteAdapter + 9);
+      if (adapted) ok = ok && mbar_wait(&d_full[turn], (i >> 1) & 1, kSiteAdapter + 6);
+      ok = __all_sync(0xffffffffu, ok);
+      uint8_t* stage = y_ring + slot * C::Y_BYTES;
+      if (adapted && !idle) {
+        tc_fence_after();
+#pragma unroll
+        for (int c = 0; c < 128; c += 32) {
+          uint32_t d[32];
+          tmem_ld32(tmem + ((uint32_t)quarter << 21) + turn * 128 + c, d);
+          tmem_wait_ld32(d);
+#pragma unroll
+          for (int e = 0; e < 32; e += 8) {
+            Raw8<T> y;
+            T* piece = reinterpret_cast<T*>(stage + (c >> 6) * (128 * 128) + row * 128 + (((((c + e) & 63) >> 3) ^ (row & 7)) << 4));
+            y.load(piece);
+            float v[8];
+            y.get(v);
+#pragma unroll
+            for (int k = 0; k < 8; ++k) v[k] = fmaf(factor, __uint_as_float(d[e + k]), v[k]);
+            y.set(v);
+            y.store(piece);
+          }
+        }
+        tc_fence_before();
+        if (box) fence_proxy_async_smem();
+      }
+      __syncwarp();
+      if (adapted && lane == 0) mbar_arrive(&d_empty[turn]);
+      if (box) {
+        if (lane == 0) {
+          for (int c = 0; c < 2; ++c)
+            if (col + 64 * c < end)
+              tma_store_2d(&tm_out, smem_u32(stage + c * (128 * 128) + quarter * (32 * 128)), col + 64 * c, order[32 * quarter]);
+          bulk_commit_group();
+          bulk_wait_group_read_1();  // the box of the step before has been read: its slot is free
+          if (sent >= 0) mbar_arrive(&y_empty[sent]);
+        }
+        sent = slot;
+      } else {
+        for (int r = 0; !idle && r < min(32, tile.z - 32 * quarter); r += 2) {  // 16 lanes a row
+          const int rr = r + (lane >> 4), piece = lane & 15;
+          const int to = __shfl_sync(0xffffffffu, mine, rr);
+          if (to < 0 || col + 8 * piece >= end) continue;
+          *reinterpret_cast<uint4*>(reinterpret_cast<T*>(p.out) + to * p.out_stride + col + 8 * piece) =
+              *reinterpret_cast<const uint4*>(stage + (piece >> 3) * (128 * 128) + (32 * quarter + rr) * 128 + (((piece & 7) ^ (rr & 7)) << 4));
+        }
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&y_empty[slot]);
+      }
+    }
+    if (box && lane == 0) bulk_wait_group_all();
+    tc_fence_before();
+  }
+  __syncthreads();
+  if (warp == kIssuer) tmem_dealloc(tmem, 256);
 }
 
 int padded_rank(int64_t R) { return R <= 16 ? 16 : R <= 32 ? 32 : R <= 64 ? 64 : 128; }
@@ -366,42 +731,104 @@ int k_slices(int64_t M, int64_t K, int64_t S, int tile, int* k_slice) {
   return (int)ceil_div(K, *k_slice);
 }
 
+// 64- or 128-column steps a CTA walks: 8 CTAs per SM and more before they get longer.
+int steps_per_cta(int64_t spans, const AdapterParams& p, int tile, int most) {
+  const int64_t tiles = ceil_div(p.M, tile) + (p.S < p.M ? p.S : p.M) / 2;
+  const int64_t steps = spans * tiles / (kSmsPlanned * 8);
+  return (int)(steps < 1 ? 1 : steps > most ? most : steps);
+}
+
 template <typename T, int TILE, int RP, bool VEC>
-cudaError_t launch_adapter(AdapterParams p, cudaStream_t stream) {
-  constexpr int WM = TILE / 16;
-  cudaError_t e = launch_pdl(adapter_shrink_kernel<T, WM, RP, VEC>, dim3(p.tiles_cap, p.slices), 128, 0, stream, p);
+cudaError_t launch_adapter(AdapterParams p, const CUtensorMap* maps, cudaStream_t stream) {
+  if constexpr (TILE == 128 && VEC) {
+    if (maps != nullptr) {
+      using C = ExpandCfg<RP>;
+      cudaError_t e = launch_pdl(adapter_shrink_kernel<T, 2, RP, VEC, true>, dim3(p.tiles_cap, 4), 256,
+                                 shrink_shared(2, RP, true), stream, p);
+      if (e != cudaSuccess) return e;
+      e = ensure_smem_limit<adapter_expand128_kernel<T, RP>>(C::SMEM);
+      if (e != cudaSuccess) return e;
+      // One CTA per SM: as many column ranges as leave the fewest steps (and CTA starts, of
+      // about two) one after the other.
+      const int64_t spans = ceil_div(p.N, 128), tiles = ceil_div(p.M, TILE) + (p.S < p.M ? p.S : p.M) / 2;
+      int64_t least = INT64_MAX;
+      for (int64_t ranges = 1; ranges <= spans && ranges <= kSmsPlanned; ++ranges) {
+        const int64_t steps = ceil_div(spans, ranges);
+        const int64_t cost = ceil_div(tiles * ranges, kSmsPlanned) * (steps + 2);
+        if (cost < least) least = cost, p.col_steps = (int)steps;
+      }
+      return launch_pdl(adapter_expand128_kernel<T, RP>, dim3((unsigned)ceil_div(spans, p.col_steps), p.tiles_cap),
+                        C::THREADS, C::SMEM, stream, maps[0], maps[1], maps[2], maps[3], p);
+    }
+  }
+  constexpr int WM = TILE == kFewRows ? 1 : TILE / 16;
+  cudaError_t e = launch_pdl(adapter_shrink_kernel<T, WM, RP, VEC, false>, dim3(p.tiles_cap, p.slices),
+                             32 * shrink_warps(WM, false), shrink_shared(WM, RP, false), stream, p);
   if (e != cudaSuccess) return e;
+  if constexpr (TILE == kFewRows && RP <= 64 && VEC) {
+    if (p.R % 8 == 0) {
+      const int64_t spans = ceil_div(p.N, 256);
+      p.col_steps = steps_per_cta(spans, p, TILE, 8);
+      return launch_pdl(adapter_expand_few_kernel<T, RP>, dim3((unsigned)ceil_div(spans, p.col_steps), p.tiles_cap), 128, 0,
+                        stream, p);
+    }
+  }
   // Two 16-row blocks per warp halve the reads of `up`; at rank 128 the split v of one
   // block already takes 64 registers.
-  constexpr int MW = TILE >= 32 && RP <= 64 ? 2 : 1;
-  constexpr int EWM = TILE / (16 * MW);
+  constexpr int MW = TILE == 128 || (TILE >= 32 && RP <= 64) ? 2 : 1;
+  constexpr int EWM = WM / MW;
   const int64_t spans = ceil_div(p.N, 64 * (4 / EWM));
-  int64_t steps = spans * ceil_div(p.M, TILE) / (kSmsPlanned * 8);
-  p.col_steps = (int)(steps < 1 ? 1 : steps > 8 ? 8 : steps);
+  p.col_steps = steps_per_cta(spans, p, TILE, 8);
   return launch_pdl(adapter_expand_kernel<T, EWM, MW, RP, VEC>, dim3((unsigned)ceil_div(spans, p.col_steps), p.tiles_cap),
                     128, 0, stream, p);
 }
 
 template <typename T, bool VEC>
-cudaError_t dispatch(const AdapterParams& p, int tile, int rp, cudaStream_t s) {
+cudaError_t dispatch(const AdapterParams& p, const CUtensorMap* maps, int tile, int rp, cudaStream_t s) {
 #define ACTUNE_ADAPTER(TILE)                                            \
   switch (rp) {                                                         \
-    case 16: return launch_adapter<T, TILE, 16, VEC>(p, s);             \
-    case 32: return launch_adapter<T, TILE, 32, VEC>(p, s);             \
-    case 64: return launch_adapter<T, TILE, 64, VEC>(p, s);             \
-    default: return launch_adapter<T, TILE, 128, VEC>(p, s);            \
+    case 16: return launch_adapter<T, TILE, 16, VEC>(p, maps, s);         \
+    case 32: return launch_adapter<T, TILE, 32, VEC>(p, maps, s);         \
+    case 64: return launch_adapter<T, TILE, 64, VEC>(p, maps, s);         \
+    default: return launch_adapter<T, TILE, 128, VEC>(p, maps, s);        \
   }
-  if (tile == 16) {
+  if (tile == kFewRows) {
+    ACTUNE_ADAPTER(kFewRows)
+  } else if (tile == 16) {
     ACTUNE_ADAPTER(16)
   } else if (tile == 32) {
     ACTUNE_ADAPTER(32)
   }
-  ACTUNE_ADAPTER(64)
+  ACTUNE_ADAPTER(128)
 #undef ACTUNE_ADAPTER
 }
 
+// [n, rows, ranks] -> boxes of 64 ranks x 128 rows, 128-byte swizzled (ranks past the end
+// read as zero).
+int encode_ranks(CUtensorMap* map, int dtype, const void* base, int64_t ranks, int64_t rows, int64_t n) {
+  const cuuint64_t dims[3] = {(cuuint64_t)ranks, (cuuint64_t)rows, (cuuint64_t)n};
+  const cuuint64_t strides[2] = {(cuuint64_t)(ranks * 2), (cuuint64_t)(rows * ranks * 2)};
+  const cuuint32_t box[3] = {64, 128, 1}, estr[3] = {1, 1, 1};
+  const CUresult r = tensor_map_encoder()(
+      map, dtype == ACTUNE_DTYPE_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 3,
+      const_cast<void*>(base), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+      CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  return r == CUDA_SUCCESS ? ACTUNE_OK : ACTUNE_ERR_CUDA;
+}
+
+// [rows, N] -> boxes of 64 columns x 32 rows, 128-byte swizzled.
+int encode_matrix(CUtensorMap* map, int dtype, const void* base, int64_t rows, int64_t N, int64_t stride) {
+  const cuuint64_t dims[2] = {(cuuint64_t)N, (cuuint64_t)rows}, strides[1] = {(cuuint64_t)(stride * 2)};
+  const cuuint32_t box[2] = {64, 32}, estr[2] = {1, 1};
+  const CUresult r = tensor_map_encoder()(
+      map, dtype == ACTUNE_DTYPE_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 2,
+      const_cast<void*>(base), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+      CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  return r == CUDA_SUCCESS ? ACTUNE_OK : ACTUNE_ERR_CUDA;
+}
+
 bool valid_plan(int64_t M, int64_t S, int tile) {
-  return M >= 0 && M <= (1 << 28) && S > 0 && S <= kMaxSlots && (tile == 16 || tile == 32 || tile == 64) &&
+  return M >= 0 && M <= (1 << 28) && S > 0 && S <= kMaxSlots && (tile == kFewRows || tile == 16 || tile == 32 || tile == 128) &&
          max_tiles(M, S, tile) <= 65535;
 }
 
@@ -431,7 +858,7 @@ int actune_adapter_plan(const int32_t* slots, int64_t M, int64_t S, int tile, in
 size_t actune_adapter_workspace_size(int64_t M, int64_t K, int64_t S, int64_t R, int tile) {
   if (!valid_plan(M, S, tile) || M == 0 || K <= 0 || K > 0x7fffff00 || R <= 0 || R > kMaxRank) return 0;
   int k_slice = 0;
-  return 4 * (size_t)k_slices(M, K, S, tile, &k_slice) * (size_t)M * (size_t)padded_rank(R);
+  return 4 * ((size_t)k_slices(M, K, S, tile, &k_slice) * (size_t)M * (size_t)padded_rank(R) + (tile == 128 ? (size_t)M : 0));
 }
 
 int actune_adapter_add(const actune_adapter_args* a, void* stream) {
@@ -465,11 +892,27 @@ int actune_adapter_add(const actune_adapter_args* a, void* stream) {
   p.slices = k_slices(a->M, a->K, a->S, a->tile, &p.k_slice);
   const int rp = padded_rank(a->R);
   auto* cs = reinterpret_cast<cudaStream_t>(stream);
+  CUtensorMap both[4] = {};
+  const CUtensorMap* maps = nullptr;
+  if (vec && a->tile == 128 && a->R % 8 == 0) {  // rows of `up` a multiple of 16 bytes, as tensor maps want them
+    p.split = a->workspace;
+    p.factor = reinterpret_cast<float*>(a->workspace) + a->M * rp;
+    int st = encode_ranks(&both[0], a->dtype, a->up, a->R, a->N, a->S);
+    if (st == ACTUNE_OK) st = encode_ranks(&both[1], a->dtype, p.split, rp, a->M, 2);
+    if (st != ACTUNE_OK) return st;
+    maps = both;
+    if (p.y_stride > 0) {
+      p.boxes = 1;
+      st = encode_matrix(&both[2], a->dtype, a->y, a->M, a->N, a->y_stride);
+      if (st == ACTUNE_OK) st = encode_matrix(&both[3], a->dtype, a->out, a->M, a->N, a->out_stride);
+      if (st != ACTUNE_OK) return st;
+    }
+  }
   cudaError_t e;
   if (a->dtype == ACTUNE_DTYPE_BF16)
-    e = vec ? dispatch<__nv_bfloat16, true>(p, a->tile, rp, cs) : dispatch<__nv_bfloat16, false>(p, a->tile, rp, cs);
+    e = vec ? dispatch<__nv_bfloat16, true>(p, maps, a->tile, rp, cs) : dispatch<__nv_bfloat16, false>(p, maps, a->tile, rp, cs);
   else
-    e = vec ? dispatch<__half, true>(p, a->tile, rp, cs) : dispatch<__half, false>(p, a->tile, rp, cs);
+    e = vec ? dispatch<__half, true>(p, maps, a->tile, rp, cs) : dispatch<__half, false>(p, maps, a->tile, rp, cs);
   return serving_status(e);
 }
 

@@ -103,14 +103,15 @@ def adapter_plan(slots, adapters):
     """Sort a batch's rows by adapter: slots int32 [M] on the GPU (row m runs adapter
     slots[m]; anything outside 0 .. adapters - 1 means none) -> AdapterPlan.
 
-    Tiles of rows that share an adapter have 16, 32 or 64 rows, by the mean number of
-    rows per adapter that the sizes allow."""
+    Tiles of rows that share an adapter have 4, 16, 32 or 128 rows, by the mean number of
+    rows per adapter that the sizes allow; a row's result depends on its own operands and
+    these sizes, not on the rows beside it."""
     _check_slots(slots)
     rows = slots.shape[0]
     if not 1 <= adapters <= 8191:
         raise RuntimeError("between 1 and 8191 adapters")
     mean = rows / min(adapters, rows) if rows else 0
-    tile = 16 if mean <= 16 else 32 if mean <= 32 else 64
+    tile = 4 if mean <= 2 else 16 if mean <= 16 else 32 if mean <= 128 else 128
     size = _lib.lib().actune_adapter_plan_size(rows, adapters, tile)
     if size == 0:
         raise RuntimeError(f"too many rows for one plan: {rows}")

@@ -94,7 +94,7 @@ def test_adapter_sizes():
     assert L.actune_adapter_plan_size(0, 3, 16) == 16
     assert L.actune_adapter_plan_size(100, 3, 8) == 0 and L.actune_adapter_plan_size(-1, 3, 16) == 0
     assert L.actune_adapter_workspace_size(1, 4096, 1, 8, 16) == 32 * 16 * 4  # 32 slices of K, rank padded to 16
-    assert L.actune_adapter_workspace_size(100000, 4096, 1, 100, 64) == 100000 * 128 * 4
+    assert L.actune_adapter_workspace_size(100000, 4096, 1, 100, 128) == 100000 * (128 + 1) * 4
     assert L.actune_adapter_workspace_size(1, 4096, 1, 129, 16) == 0
 
 
