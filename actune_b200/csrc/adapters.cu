@@ -175,7 +175,7 @@ __device__ __forceinline__ void split2(float a, float b, uint32_t& hi, uint32_t&
 // of rows g and g + 8 of x and of row g of each 8-row block of down, two MMAs per block.
 // Nothing is shared between warps until their sums are added in shared memory.
 //
-// SPLIT: a quarter of a 128-row tile and all of K, 8 warps; the sums are complete, and go
+// SPLIT: 16 rows of a 128-row tile and all of K, 8 warps; the sums are complete, and go
 // out as the two 16-bit parts that the next kernel takes.  Else a tile and one slice of K;
 // the slice's sums go out in fp32.
 constexpr int shrink_warps(int wm, bool split) { return split || wm > 4 ? 8 : 4; }
@@ -664,22 +664,28 @@ __global__ void __launch_bounds__(ExpandCfg<RP>::THREADS, 1)
       uint8_t* stage = y_ring + slot * C::Y_BYTES;
       if (adapted && !idle) {
         tc_fence_after();
+        const uint32_t d_at = tmem + ((uint32_t)quarter << 21) + turn * 128;
+        uint32_t d[2][32];
+        tmem_ld32(d_at, d[0]);
 #pragma unroll
-        for (int c = 0; c < 128; c += 32) {
-          uint32_t d[32];
-          tmem_ld32(tmem + ((uint32_t)quarter << 21) + turn * 128 + c, d);
-          tmem_wait_ld32(d);
+        for (int c = 0; c < 4; ++c) {  // 32 columns: the next accumulators are read under this sum
+          T* piece[4];
+          Raw8<T> y[4];
 #pragma unroll
-          for (int e = 0; e < 32; e += 8) {
-            Raw8<T> y;
-            T* piece = reinterpret_cast<T*>(stage + (c >> 6) * (128 * 128) + row * 128 + (((((c + e) & 63) >> 3) ^ (row & 7)) << 4));
-            y.load(piece);
+          for (int e = 0; e < 4; ++e) {
+            piece[e] = reinterpret_cast<T*>(stage + (c >> 1) * (128 * 128) + row * 128 + (((4 * (c & 1) + e) ^ (row & 7)) << 4));
+            y[e].load(piece[e]);
+          }
+          tmem_wait_ld32(d[c & 1]);
+          if (c < 3) tmem_ld32(d_at + 32 * (c + 1), d[(c + 1) & 1]);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
             float v[8];
-            y.get(v);
+            y[e].get(v);
 #pragma unroll
-            for (int k = 0; k < 8; ++k) v[k] = fmaf(factor, __uint_as_float(d[e + k]), v[k]);
-            y.set(v);
-            y.store(piece);
+            for (int k = 0; k < 8; ++k) v[k] = fmaf(factor, __uint_as_float(d[c & 1][8 * e + k]), v[k]);
+            y[e].set(v);
+            y[e].store(piece[e]);
           }
         }
         tc_fence_before();
@@ -743,20 +749,17 @@ cudaError_t launch_adapter(AdapterParams p, const CUtensorMap* maps, cudaStream_
   if constexpr (TILE == 128 && VEC) {
     if (maps != nullptr) {
       using C = ExpandCfg<RP>;
-      cudaError_t e = launch_pdl(adapter_shrink_kernel<T, 2, RP, VEC, true>, dim3(p.tiles_cap, 4), 256,
-                                 shrink_shared(2, RP, true), stream, p);
+      cudaError_t e = ensure_smem_limit<adapter_shrink_kernel<T, 1, RP, VEC, true>>(shrink_shared(1, RP, true));
+      if (e != cudaSuccess) return e;
+      e = launch_pdl(adapter_shrink_kernel<T, 1, RP, VEC, true>, dim3(p.tiles_cap, 8), 256,
+                                 shrink_shared(1, RP, true), stream, p);
       if (e != cudaSuccess) return e;
       e = ensure_smem_limit<adapter_expand128_kernel<T, RP>>(C::SMEM);
       if (e != cudaSuccess) return e;
-      // One CTA per SM: as many column ranges as leave the fewest steps (and CTA starts, of
-      // about two) one after the other.
-      const int64_t spans = ceil_div(p.N, 128), tiles = ceil_div(p.M, TILE) + (p.S < p.M ? p.S : p.M) / 2;
-      int64_t least = INT64_MAX;
-      for (int64_t ranges = 1; ranges <= spans && ranges <= kSmsPlanned; ++ranges) {
-        const int64_t steps = ceil_div(spans, ranges);
-        const int64_t cost = ceil_div(tiles * ranges, kSmsPlanned) * (steps + 2);
-        if (cost < least) least = cost, p.col_steps = (int)steps;
-      }
+      // One CTA per SM; up to 16 steps a CTA, so that tiles of few rows and of many even out
+      // (40 x 150 rows 1024 -> 8192: 82 us, 106 us with 64 steps).
+      const int64_t spans = ceil_div(p.N, 128);
+      p.col_steps = steps_per_cta(2 * spans, p, TILE, 16);
       return launch_pdl(adapter_expand128_kernel<T, RP>, dim3((unsigned)ceil_div(spans, p.col_steps), p.tiles_cap),
                         C::THREADS, C::SMEM, stream, maps[0], maps[1], maps[2], maps[3], p);
     }
@@ -768,7 +771,7 @@ cudaError_t launch_adapter(AdapterParams p, const CUtensorMap* maps, cudaStream_
   if constexpr (TILE == kFewRows && RP <= 64 && VEC) {
     if (p.R % 8 == 0) {
       const int64_t spans = ceil_div(p.N, 256);
-      p.col_steps = steps_per_cta(spans, p, TILE, 8);
+      p.col_steps = RP == 16 ? (steps_per_cta(2 * spans, p, TILE, 8) + 1) / 2 * 2 : steps_per_cta(spans, p, TILE, 8);
       return launch_pdl(adapter_expand_few_kernel<T, RP>, dim3((unsigned)ceil_div(spans, p.col_steps), p.tiles_cap), 128, 0,
                         stream, p);
     }

@@ -1,0 +1,82 @@
+"""Adapter slots and scopes on the CPU: installing, loading, refusals, pass-through."""
+import pytest
+import torch
+
+from actune_b200.adapters import AdaptedLinear, active_adapter_plan, adapter_scope, install_adapters
+
+
+def model():
+    m = torch.nn.Module()
+    m.block = torch.nn.Module()
+    m.block.up = torch.nn.Linear(12, 20, dtype=torch.bfloat16)
+    m.block.down = torch.nn.Linear(20, 12, bias=False, dtype=torch.bfloat16)
+    return m
+
+
+def test_install_wraps_the_named_projections_and_passes_through_without_a_scope():
+    m = model()
+    before = m.block.up
+    x = torch.randn(3, 12).bfloat16()
+    want = before(x)
+    adapted = install_adapters(m, ["block.up", "block.down"], slots=4, rank=6)
+    assert m.block.up is adapted["block.up"] and m.block.up.projection is before
+    assert torch.equal(m.block.up(x), want)
+    assert m.block.up.in_features == 12 and m.block.up.out_features == 20 and m.block.up.weight is before.weight
+    # the rank is held in whole 16-byte rows
+    assert m.block.up.down.shape == (4, 8, 12) and m.block.up.up.shape == (4, 20, 8)
+    assert m.block.up.padding == 0 and m.block.up.input_scale is None and not hasattr(m.block.up, "active_backend")
+
+
+def test_install_checks_everything_before_touching_the_model():
+    m = model()
+    m.block.act = torch.nn.ReLU()
+    with pytest.raises(ValueError, match="block.act"):
+        install_adapters(m, ["block.up", "block.act"], 4, 8)
+    assert isinstance(m.block.up, torch.nn.Linear)
+    install_adapters(m, ["block.up"], 4, 8)
+    with pytest.raises(ValueError, match="block.up"):
+        install_adapters(m, ["block.up"], 4, 8)
+    for slots, rank in ((0, 8), (9000, 8), (4, 0), (4, 129)):
+        with pytest.raises(ValueError, match="slots"):
+            install_adapters(m, ["block.down"], slots, rank)
+    with pytest.raises(ValueError, match="float16 or bfloat16"):
+        install_adapters(m, ["block.down"], 4, 8, dtype=torch.float32)
+
+
+def test_load_and_clear_a_slot():
+    a = AdaptedLinear(torch.nn.Linear(12, 20), slots=2, rank=6)
+    down, up = torch.randn(4, 12), torch.randn(20, 4)
+    a.load(1, torch.ones(6, 12), torch.ones(20, 6), 3.0)
+    a.load(1, down, up, 0.5)  # replaces all of the earlier one
+    assert torch.equal(a.down[1, :4], down.bfloat16()) and not a.down[1, 4:].any()
+    assert torch.equal(a.up[1, :, :4], up.bfloat16()) and not a.up[1, :, 4:].any()
+    assert a.scale.tolist() == [0.0, 0.5] and not a.down[0].any()
+    a.clear(1)
+    assert not a.down.any() and not a.up.any() and not a.scale.any()
+    for slot, d, u in ((2, down, up), (-1, down, up), (0, torch.zeros(7, 12), torch.zeros(20, 7)),
+                       (0, down[:, :11], up), (0, down, up[:19]), (0, down[:0], up[:, :0])):
+        with pytest.raises(ValueError):
+            a.load(slot, d, u)
+
+
+def test_scope_is_nested_and_restored():
+    plan, other = object(), object()
+    assert active_adapter_plan() is None
+    with adapter_scope(plan):
+        with adapter_scope(other):
+            assert active_adapter_plan() is other
+        with adapter_scope(None):
+            assert active_adapter_plan() is None
+        assert active_adapter_plan() is plan
+    assert active_adapter_plan() is None
+
+
+def test_a_bank_projection_keeps_its_format():
+    class Resident(torch.nn.Linear):
+        padding, input_scale = 4, None
+
+        def active_backend(self):
+            return "backend"
+
+    a = AdaptedLinear(Resident(12, 20), slots=1, rank=8)
+    assert a.padding == 4 and hasattr(a, "active_backend") and a.active_backend() == "backend"
