@@ -105,7 +105,7 @@ def _declare(L):
     L.actune_adapter_plan.argtypes = [p, i64, i64, i32, p, p]
     L.actune_adapter_workspace_size.argtypes = [i64, i64, i64, i64, i32]
     L.actune_adapter_add.argtypes = [p, p]
-    L.actune_prefix_attention_workspace_size.argtypes = [i64] * 8
+    L.actune_prefix_attention_workspace_size.argtypes = [i64] * 8 + [i32]
     L.actune_prefix_attention.argtypes = [p, p]
     for name in EXPORTS + SERVING_EXPORTS:
         if name.endswith("_size"):

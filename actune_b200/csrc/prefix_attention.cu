@@ -8,15 +8,18 @@
 // (s in units of log2).  Parts of the keys computed apart are joined by the same rule.
 //
 // A work item is a tile of 128 (or 2 x 128) query rows of one key/value head and a range
-// of 128 keys (64 at head sizes above 128) at a time.  There are two ways to make tiles:
+// of 128 keys (64 at head sizes above 128) at a time.  There are three ways to make tiles:
 //   * by sequence: the rows (token, query head of the group) of one sequence against its
 //     prefix and then its own keys.  One launch when there are tiles enough.
 //   * stacked: for the prefix, the rows of all sequences that share it are stacked, so a
 //     prefix is read once for the batch and not once per sequence; each sequence's own
-//     keys are a further item, and the parts are joined by a second kernel.
-// Either way the key range is split over more items when tiles are few.  A tile never
-// holds rows of one sequence and keys of another's own, so no value of one request
-// enters another's sums, not even multiplied by zero.
+//     keys are a further item, and the parts are joined by a second kernel.  For few
+//     query rows, whose own keys need the tiles' rows for little.
+//   * mixed: stacked tiles that go through the prefix and then through the own keys of
+//     each of their sequences, the product with V writing that sequence's rows alone.
+//     For tiles of few sequences, when there are tiles enough: no parts to join.
+// In the first two the key range is split over more items when tiles are few.  No value
+// of one request enters another's sums, not even multiplied by zero.
 //
 // One item per CTA:
 //   softmax warps   4 per 128 rows, thread = row: scores from tensor memory to registers,
@@ -36,6 +39,11 @@ namespace {
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kRescale = 8.f;  // growth of the maximum (log2) that O is rescaled for
 constexpr int kSiteAttn = 300;
+
+// Tiles by sequence; stacked tiles for the prefix and tiles by sequence for the own keys;
+// stacked tiles for both.
+enum : int { kBySequence = 0, kStacked = 1, kMixed = 2 };
+constexpr int kMixedSeqs = 16;  // sequences that a mixed tile may touch
 
 // n / d for 0 <= n < 2^31 by multiplication: an item's place in the grid and a row's
 // place in its sequence are several divisions deep before the first load can start.
@@ -67,7 +75,7 @@ struct AttnParams {
   int causal;
   float scale;      // scale * log2(e)
   int tiles_per_seq;
-  int stacked;      // 0: tiles by sequence; 1: stacked prefix tiles, then own-key tiles
+  int kind;         // how tiles are made: kBySequence, kStacked or kMixed
   int prefix_tiles; // upper bound on the stacked tiles of a key/value head
   int prefix_splits, own_splits;  // by sequence: prefix_splits of both together
   int splits;       // parts per row; 1: write out directly
@@ -160,6 +168,17 @@ __device__ __forceinline__ void mma16_ts(uint32_t d, uint32_t a, uint64_t b, uin
       : "memory");
 }
 
+// The same, leaving the accumulator's rows whose bit of `off` is set as they are.
+__device__ __forceinline__ void mma16_ts_rows(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t acc,
+                                              const uint32_t (&off)[4]) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, {%5, %6, %7, %8}, p;\n\t}" ::"r"(d),
+      "r"(a), "l"(b), "r"(idesc), "r"(acc), "r"(off[0]), "r"(off[1]), "r"(off[2]), "r"(off[3])
+      : "memory");
+}
+
 // MN-major operand in 128-byte-swizzled tiles of 64 columns x `rows` rows (128 bytes a
 // row, 8-row atoms of 1024 bytes): LBO = the next 64 columns, SBO = the next 8 rows.
 __device__ __forceinline__ uint64_t smem_desc_mn_sw128(uint32_t saddr, uint32_t rows) {
@@ -229,6 +248,14 @@ struct AttnCfg {
   static_assert(S_COL + NT * NB * BN <= TMEM_COLS && RING >= 2 && SMEM + NT * 1024 + 512 <= 227 * 1024, "fits");
 };
 
+// A mixed tile's sequences seq0 .. seq0 + count - 1 (those with rows in it), by index.
+struct TileSeqs {
+  int count;
+  int row[kMixedSeqs + 1];    // first row in the tile; the last entry is the end
+  int block[kMixedSeqs + 1];  // first of the sequence's own blocks, counted over the tile's
+  int len[kMixedSeqs];        // own keys
+};
+
 struct AttnItem {
   int nrows;         // rows of the tile; 0: nothing to do
   int row0;          // first row, counted from sequence seq0: ((b - seq0) * T + t) * rep + r
@@ -239,12 +266,12 @@ struct AttnItem {
 };
 
 // What the CTA works on; by one warp.
-template <int BN, int ROWS>
-__device__ AttnItem attn_item(const AttnParams& p, int lane) {
+template <int BN, int ROWS, bool MIXED>
+__device__ AttnItem attn_item(const AttnParams& p, int lane, TileSeqs& seqs) {
   AttnItem it = {};
   const int per_seq = p.T * p.rep;
   int x = blockIdx.x;
-  const int prefix_items = p.stacked ? p.prefix_tiles * p.KV * p.prefix_splits : 0;
+  const int prefix_items = p.kind != kBySequence ? p.prefix_tiles * p.KV * p.prefix_splits : 0;
   // Part `i` of `blocks` blocks dealt to d.d parts: [begin, end).
   const auto deal = [](int blocks, const Divisor& d, int i, int& begin, int& end) {
     int each = blocks;
@@ -292,6 +319,35 @@ __device__ AttnItem attn_item(const AttnParams& p, int lane) {
     if (!found) return it;
     it.b = it.seq0;
     it.plen = clamp_len(p.prefix_lens, it.g, p.P);
+    if constexpr (MIXED) {
+      // The tile's first sequence becomes seq0, and a lane works out each sequence's share.
+      const int skip = p.by_per_seq.div(it.row0);
+      it.seq0 += skip, it.b = it.seq0, it.row0 -= skip * per_seq;
+      const int count = p.by_per_seq.div(it.row0 + it.nrows - 1) + 1;
+      int blocks = 0, len = 0, begin = it.nrows;
+      if (lane < count) {
+        len = clamp_len(p.lens, it.seq0 + lane, p.S);
+        begin = max(0, lane * per_seq - it.row0);
+        int seen = len;  // by the sequence's last row in the tile
+        if (p.causal) {
+          const int last = min((lane + 1) * per_seq, it.row0 + it.nrows) - 1 - lane * per_seq;
+          seen = max(0, min(len, len - p.T + p.by_rep.div(last) + 1));
+        }
+        blocks = (seen + BN - 1) / BN;
+      }
+      int upto = blocks;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const int a = __shfl_up_sync(0xffffffffu, upto, o);
+        if (lane >= o) upto += a;
+      }
+      if (lane == 0) seqs.count = count;
+      if (lane <= count && lane <= kMixedSeqs) seqs.row[lane] = begin, seqs.block[lane] = upto - blocks;
+      if (lane < count && lane < kMixedSeqs) seqs.len[lane] = len;
+      it.pb1 = (it.plen + BN - 1) / BN;
+      it.sb1 = __shfl_sync(0xffffffffu, upto, 31);
+      return it;
+    }
     deal((it.plen + BN - 1) / BN, p.by_prefix_splits, it.split, it.pb0, it.pb1);
     return it;
   }
@@ -306,7 +362,7 @@ __device__ AttnItem attn_item(const AttnParams& p, int lane) {
   int seen = it.slen;  // own keys that the tile's last row sees
   if (p.causal) seen = max(0, min(seen, it.slen - p.T + p.by_rep.div(it.row0 + it.nrows - 1) + 1));
   const int own = (seen + BN - 1) / BN;
-  if (p.stacked) {
+  if (p.kind == kStacked) {
     it.split = p.prefix_splits + part;
     deal(own, p.by_own_splits, part, it.sb0, it.sb1);
     return it;
@@ -329,7 +385,8 @@ __device__ AttnItem attn_item(const AttnParams& p, int lane) {
   return it;
 }
 
-template <typename T, int DP, int NT>
+// (MIXED a parameter of the kernel: carried along, its tests cost the others 2-4%.)
+template <typename T, int DP, int NT, bool MIXED>
 __global__ void __launch_bounds__(AttnCfg<DP, NT>::WARPS * 32, 1)
     prefix_attention_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUtensorMap tm_pk, const __grid_constant__ CUtensorMap tm_pv,
                             const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CUtensorMap tm_v,
@@ -342,6 +399,7 @@ __global__ void __launch_bounds__(AttnCfg<DP, NT>::WARPS * 32, 1)
   __shared__ __align__(8) uint64_t full[RING], empty[RING], step[NT][NB], p_ready[NT][NB], drained[NT], q_full[NT];
   __shared__ uint32_t tmem_holder;
   __shared__ AttnItem item_sh;
+  __shared__ TileSeqs seqs;
   __shared__ float pair_sh[2][C::ROWS];  // a row's two threads: maxima, at the end sums
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
@@ -376,7 +434,7 @@ __global__ void __launch_bounds__(AttnCfg<DP, NT>::WARPS * 32, 1)
   }
   griddep_enter();
   if (warp == kProducer) {
-    const AttnItem it = attn_item<BN, C::ROWS>(p, lane);
+    const AttnItem it = attn_item<BN, C::ROWS, MIXED>(p, lane, seqs);
     if (lane == 0) item_sh = it;
   }
   tc_fence_before();
@@ -405,6 +463,7 @@ __global__ void __launch_bounds__(AttnCfg<DP, NT>::WARPS * 32, 1)
         }
       }
       int issued = 0;
+      int of[2] = {0, 0};  // mixed tiles: the sequence K and V are at
       for (int j = 0; j < stages; ++j) {
         const int slot = j % RING;
         if (j >= RING && !mbar_wait(&empty[slot], (j / RING - 1) & 1, kSiteAttn)) break;
@@ -414,7 +473,11 @@ __global__ void __launch_bounds__(AttnCfg<DP, NT>::WARPS * 32, 1)
           if (i < 0 || i >= nblk) continue;
           const bool prefix = i < np;
           const CUtensorMap* map = prefix ? (is_v ? &tm_pv : &tm_pk) : (is_v ? &tm_v : &tm_k);
-          const int key = (prefix ? it.pb0 + i : it.sb0 + i - np) * BN, who = prefix ? it.g : it.b;
+          int key = (prefix ? it.pb0 + i : it.sb0 + i - np) * BN, who = prefix ? it.g : it.b;
+          if (MIXED && !prefix) {
+            while (i - np >= seqs.block[of[is_v] + 1]) ++of[is_v];
+            key = (i - np - seqs.block[of[is_v]]) * BN, who = it.seq0 + of[is_v];
+          }
           const uint32_t at = smem_u32(ring) + slot * C::STAGE_BYTES + is_v * C::SLOT_BYTES;
 #pragma unroll
           for (int c = 0; c < DP / 64; ++c) tma_load_4d(at + c * BN * 128, map, 64 * c, it.kv, key, who, smem_u32(&full[slot]));
@@ -452,6 +515,7 @@ __global__ void __launch_bounds__(AttnCfg<DP, NT>::WARPS * 32, 1)
       ok = mbar_wait(&q_full[t], 0, kSiteAttn + 2);
       int buffer = 0;
       uint32_t turn = 0;  // p_ready's phase
+      int of = 0;         // mixed tiles: the sequence V is at
       for (int i = -NB; i < nblk && ok; ++i) {
         // O += P(i) V(i), then S(i + NB) = Q K^T over the p just taken.
         const uint32_t s_at = s_col + buffer * BN;
@@ -461,10 +525,28 @@ __global__ void __launch_bounds__(AttnCfg<DP, NT>::WARPS * 32, 1)
         tc_fence_after();
         if (i >= 0) {
           const uint64_t v_desc = v_desc0 + (uint32_t)slot * kStageStep;
+          // Each half of the keys has its p over its own scores.
+          const auto p_at = [&](int k) { return s_at + (k / (BN / 32)) * (BN / 2) + (k % (BN / 32)) * 8; };
+          if (MIXED && i >= np) {
+            // Own keys of one sequence: rows of the others keep their O, whatever p and V hold.
+            while (i - np >= seqs.block[of + 1]) ++of;
+            const bool add = np > 0 || i - np > seqs.block[of];
+            uint32_t off[4];
 #pragma unroll
-          for (int k = 0; k < BN / 16; ++k)  // each half of the keys has its p over its own scores
-            mma16_ts(o_col, s_at + (k / (BN / 32)) * (BN / 2) + (k % (BN / 32)) * 8, v_desc + k * (2048 / 16),
-                     idesc_16<T>(DP, true), i > 0 || k > 0);
+            for (int w = 0; w < 4; ++w) {
+              const int lo = seqs.row[of] - t * 128 - 32 * w, hi = seqs.row[of + 1] - t * 128 - 32 * w;
+              const uint32_t below = lo <= 0 ? 0u : lo >= 32 ? ~0u : (1u << lo) - 1u;
+              const uint32_t upto = hi <= 0 ? 0u : hi >= 32 ? ~0u : (1u << hi) - 1u;
+              off[w] = ~(upto & ~below);
+            }
+#pragma unroll
+            for (int k = 0; k < BN / 16; ++k)
+              mma16_ts_rows(o_col, p_at(k), v_desc + k * (2048 / 16), idesc_16<T>(DP, true), add || k > 0, off);
+          } else {
+#pragma unroll
+            for (int k = 0; k < BN / 16; ++k)
+              mma16_ts(o_col, p_at(k), v_desc + k * (2048 / 16), idesc_16<T>(DP, true), i > 0 || k > 0);
+          }
         }
         if (i + NB < nblk) scores(s_at);
         mma_commit(&step[t][buffer]);
@@ -492,6 +574,7 @@ __global__ void __launch_bounds__(AttnCfg<DP, NT>::WARPS * 32, 1)
     int head = p.by_per_seq.split(b);  // row of its sequence: token * rep + head of the group
     int tok = head;
     head = it.kv * p.rep + p.by_rep.split(tok);
+    const int my_seq = b;  // among the tile's
     b += it.seq0;
     const bool live = my < it.nrows;
     if (nblk > 0 && !p.q_boxes) {
@@ -513,8 +596,9 @@ __global__ void __launch_bounds__(AttnCfg<DP, NT>::WARPS * 32, 1)
       __syncwarp();
       if (lane == 0) mbar_arrive(&q_full[t]);
     }
-    int own_end = it.slen;  // own keys this row sees
-    if (p.causal) own_end = max(0, min(it.slen, it.slen - p.T + tok + 1));
+    const int my_len = MIXED ? (live ? seqs.len[my_seq] : 0) : it.slen;
+    int own_end = my_len;  // own keys this row sees
+    if (p.causal) own_end = max(0, min(my_len, my_len - p.T + tok + 1));
     const bool idle = t * 128 + (warp & 3) * 32 >= it.nrows;
     float m = -INFINITY, l = 0.f;
     const uint32_t o_addr = tmem + lanes + C::O_COL + t * DP;
@@ -524,7 +608,9 @@ __global__ void __launch_bounds__(AttnCfg<DP, NT>::WARPS * 32, 1)
     // Blocks that hold keys some row of the warp does not see: the prefix's last if it is
     // not full, and the own ones from own_mask on.
     const int mask_prefix = np > 0 && (int64_t)it.pb1 * BN > it.plen ? np - 1 : -1;
-    const int own_mask = np + max(0, (int)__reduce_min_sync(0xffffffffu, own_end) / BN - it.sb0);
+    const int own_mask =
+        MIXED ? np : np + max(0, (int)__reduce_min_sync(0xffffffffu, own_end) / BN - it.sb0);
+    int of = 0;  // mixed tiles: the sequence the block belongs to
     int buffer = 0;
     uint32_t turn = 0;
     for (int i = 0; i < nblk; ++i) {
@@ -532,15 +618,26 @@ __global__ void __launch_bounds__(AttnCfg<DP, NT>::WARPS * 32, 1)
       ok = __all_sync(0xffffffffu, ok);
       const bool masked = i == mask_prefix || i >= own_mask;
       int end = BN;  // keys of this half that the row sees
+      bool idle_here = idle;
       if (masked) {
         const bool prefix = i < np;
-        const int key = (prefix ? it.pb0 + i : it.sb0 + i - np) * BN;
-        end = (prefix ? it.plen : own_end) - key - half * HALF;
+        int key = (prefix ? it.pb0 + i : it.sb0 + i - np) * BN;
+        int len = prefix ? it.plen : my_len, sees = prefix ? it.plen : own_end;
+        if (MIXED && !prefix) {
+          while (i - np >= seqs.block[of + 1]) ++of;
+          key = (i - np - seqs.block[of]) * BN, len = seqs.len[of];
+          const bool its = live && my_seq == of;
+          if (!its) sees = 0;
+          // No row of this warp is the sequence's: its p are for nobody.  (One that is, but
+          // sees none of the block, needs zeros.)
+          idle_here = idle || !__any_sync(0xffffffffu, its);
+        }
+        end = sees - key - half * HALF;
         // Cache rows past the length may hold anything, and p = 0 would not hide a NaN.
         // (Each tile clears them before its own product; the second time changes nothing.
         // The step above says that this stage's last use is over, so that its next phase is
         // the one waited for.)
-        const int filled = (prefix ? it.plen : it.slen) - key;
+        const int filled = len - key;
         if (filled < BN && key + filled < (prefix ? p.P : p.S)) {
           const int j = i + NB;
           ok = ok && mbar_wait(&full[j % RING], (j / RING) & 1, kSiteAttn + 5);
@@ -555,11 +652,11 @@ __global__ void __launch_bounds__(AttnCfg<DP, NT>::WARPS * 32, 1)
       }
       const uint32_t s_addr = s_addr0 + buffer * BN;
       uint32_t x[32], pk[16];
-      if (!idle) {
+      if (!idle_here) {
         tc_fence_after();
         tmem_ld32(s_addr, x);
       }
-      if (!idle) {  // else: whatever these rows' p hold stays in them
+      if (!idle_here) {  // else: whatever these rows' p hold stays in them
         tmem_wait_ld32(x);
         if (masked) {
 #pragma unroll
@@ -614,7 +711,7 @@ __global__ void __launch_bounds__(AttnCfg<DP, NT>::WARPS * 32, 1)
           if (grown) m = both;
         }
       }
-      if (!idle) {
+      if (!idle_here) {
         tmem_st16(s_addr, pk);  // two to a column, over this half's scores
         tmem_wait_st();
         tc_fence_before();
@@ -750,55 +847,71 @@ __global__ void __launch_bounds__(128) prefix_attention_join_kernel(const AttnPa
 // ------------------------------------------------------------------ host
 struct AttnPlan {
   int dp, nt, bn;
-  int stacked, tiles_per_seq, prefix_tiles, prefix_splits, own_splits, splits;
+  int kind, tiles_per_seq, prefix_tiles, prefix_splits, own_splits, splits;
   int64_t items;
 };
 
 constexpr int kSmsPlanned = 148;  // B200; the workspace is sized before a device is known
 
-// How a call is cut into items, from its sizes alone.  Both ways of making tiles are
-// priced in key blocks on the busiest SM (plus, where parts have to be joined, the
-// second kernel and the parts' traffic, about three blocks), and the cheaper one is taken.
-AttnPlan attn_plan(int64_t B, int64_t T, int64_t H, int64_t KV, int64_t D, int64_t G, int64_t P, int64_t S) {
+// How a call is cut into items, from its sizes alone: the ways of making tiles are priced
+// in key blocks on the busiest SM, and the cheapest one is taken.
+AttnPlan attn_plan(int64_t B, int64_t T, int64_t H, int64_t KV, int64_t D, int64_t G, int64_t P, int64_t S,
+                   bool ragged) {
   AttnPlan best = {};
   int64_t best_cost = INT64_MAX;
   const int64_t rep = H / KV, per_seq = T * rep;
   const int dp = D <= 64 ? 64 : D <= 128 ? 128 : 256;
-  constexpr int64_t kJoin = 3, kStart = 2;  // in blocks: joining parts; a CTA's prologue and epilogue
-  for (int stacked = 0; stacked < 2; ++stacked) {
-    if (stacked && (P == 0 || B == G)) continue;  // nothing to stack
-    const int64_t rows = stacked ? ceil_div(B, G) * per_seq : per_seq;
+  const int bn = 64;  // AttnCfg::BN
+  const int64_t pb = ceil_div(P, bn), ob = ceil_div(S, bn);
+  // Eighths of a microsecond, as measured: a block of 64 keys for two row tiles of 128, for
+  // one (head size 256, smaller), and a CTA's prologue and epilogue; the second kernel, and
+  // the parts written and read at the copy rate.
+  constexpr int64_t kStart = 24, kMost = 64;
+  const auto join = [&](int64_t splits) { return splits > 1 ? 24 + splits * B * T * H * D * 8 / 800000 : 0; };
+  for (int kind = kBySequence; kind <= kMixed; ++kind) {
+    if (kind != kBySequence && (P == 0 || B == G)) continue;  // nothing to stack
+    const int64_t rows = kind != kBySequence ? ceil_div(B, G) * per_seq : per_seq;
     const int nt = dp <= 128 && rows > 128 ? 2 : 1;
-    const int64_t tile = 128 * nt;
-    const int bn = 64;  // AttnCfg::BN
-    const int64_t pb = ceil_div(P, bn), ob = ceil_div(S, bn);
+    const int64_t tile = 128 * nt, block = nt == 2 ? 9 : dp == 256 ? 8 : 6;
     AttnPlan c = {};
-    c.dp = dp, c.nt = nt, c.bn = bn, c.stacked = stacked;
+    c.dp = dp, c.nt = nt, c.bn = bn, c.kind = kind;
     c.tiles_per_seq = (int)ceil_div(per_seq, tile);
+    c.prefix_tiles = kind != kBySequence ? (int)(B * per_seq / tile + G) : 0;
     const int64_t own_tiles = B * c.tiles_per_seq * KV;
-    int64_t cost;
-    if (!stacked) {
+    // Uneven groups leave up to a part of a tile each.
+    const int64_t tiles = (ragged ? c.prefix_tiles : G * ceil_div(ceil_div(B, G) * per_seq, tile)) * KV;
+    const auto waves = [&](int64_t items, int64_t blocks) {
+      return ceil_div(items, kSmsPlanned) * (blocks * block + kStart);
+    };
+    int64_t cost = INT64_MAX;
+    if (kind == kBySequence) {
       const int64_t all = pb + ob > 0 ? pb + ob : 1;
-      int64_t splits = kSmsPlanned / own_tiles;
-      splits = splits > all / 2 ? all / 2 : splits;
-      splits = splits > 64 ? 64 : splits < 1 ? 1 : splits;
-      c.prefix_splits = c.splits = (int)splits;
-      c.items = own_tiles * splits;
-      cost = ceil_div(c.items, kSmsPlanned) * (ceil_div(all, splits) + kStart) * nt + (splits > 1 ? kJoin : 0);
-    } else {
-      c.prefix_tiles = (int)(B * per_seq / tile + G);
-      const int64_t tiles = ceil_div(B * per_seq, tile) * KV;
-      // Blocks per item that fill one wave.
-      const int64_t blocks = tiles * pb + own_tiles * ob;
-      int64_t each = ceil_div(blocks, kSmsPlanned);
+      for (int64_t n = 1; n <= kMost && n <= (all + 1) / 2; ++n) {
+        const int64_t t = waves(own_tiles * n, ceil_div(all, n)) + join(n);
+        if (t < cost) cost = t, c.prefix_splits = c.splits = (int)n;
+      }
+      c.items = own_tiles * c.splits;
+    } else if (kind == kStacked) {
+      // Blocks per item that fill one wave, prefix and own keys together.  (More parts than
+      // that measured slower: 8 single tokens behind 4096, 22 us with 10 + 2 parts, 30 us
+      // with 18 + 1.)
+      const int64_t even = ceil_div(B * per_seq, tile) * KV;
+      int64_t each = ceil_div(even * pb + own_tiles * ob, kSmsPlanned);
       each = each < 2 ? 2 : each;
-      int64_t ps = ceil_div(pb, each), os = S > 0 ? ceil_div(ob, each) : 0;
-      ps = ps > 64 ? 64 : ps, os = os > 16 ? 16 : os;
-      c.prefix_splits = (int)ps, c.own_splits = (int)os;
-      c.splits = (int)(ps + os);
-      c.items = (int64_t)c.prefix_tiles * KV * ps + own_tiles * os;
-      cost = (ceil_div(tiles * ps * (ceil_div(pb, ps) + kStart) +
-                       (os > 0 ? own_tiles * os * (ceil_div(ob, os) + kStart) : 0), kSmsPlanned)) * nt + kJoin;
+      int64_t n = ceil_div(pb, each), os = S > 0 ? ceil_div(ob, each) : 0;
+      n = n > kMost ? kMost : n, os = os > 16 ? 16 : os;
+      c.prefix_splits = (int)n;
+      cost = (even * n * (ceil_div(pb, n) * block + kStart) +
+              (os > 0 ? own_tiles * os * (ceil_div(ob, os) * block + kStart) : 0)) / kSmsPlanned + kStart + join(n + os);
+      c.own_splits = (int)os;
+      c.splits = (int)(c.prefix_splits + os);
+      c.items = (int64_t)c.prefix_tiles * KV * c.prefix_splits + own_tiles * os;
+    } else {
+      const int64_t touched = (tile - 1) / per_seq + 2;  // sequences a tile may touch
+      if (touched > kMixedSeqs) continue;
+      c.prefix_splits = c.splits = 1;
+      c.items = (int64_t)c.prefix_tiles * KV;
+      cost = waves(tiles, pb + (tile / per_seq + 1) * ob);
     }
     if (cost < best_cost) best_cost = cost, best = c;
   }
@@ -839,13 +952,19 @@ bool map_stride(int64_t* stride, int64_t extent) {
   return *stride > 0 && *stride % 8 == 0 && *stride < ((int64_t)1 << 39);
 }
 
+template <typename T, int DP, int NT, bool MIXED>
+cudaError_t launch_attn_as(const CUtensorMap (&m)[5], const AttnParams& p, int64_t items, cudaStream_t stream) {
+  using C = AttnCfg<DP, NT>;
+  const cudaError_t e = ensure_smem_limit<prefix_attention_kernel<T, DP, NT, MIXED>>(C::SMEM);
+  if (e != cudaSuccess) return e;
+  return launch_pdl(prefix_attention_kernel<T, DP, NT, MIXED>, dim3((unsigned)items), C::WARPS * 32, C::SMEM, stream,
+                    m[0], m[1], m[2], m[3], m[4], p);
+}
+
 template <typename T, int DP, int NT>
 cudaError_t launch_attn(const CUtensorMap (&m)[5], const AttnParams& p, int64_t items, cudaStream_t stream) {
-  using C = AttnCfg<DP, NT>;
-  const cudaError_t e = ensure_smem_limit<prefix_attention_kernel<T, DP, NT>>(C::SMEM);
-  if (e != cudaSuccess) return e;
-  return launch_pdl(prefix_attention_kernel<T, DP, NT>, dim3((unsigned)items), C::WARPS * 32, C::SMEM, stream, m[0],
-                    m[1], m[2], m[3], m[4], p);
+  return p.kind == kMixed ? launch_attn_as<T, DP, NT, true>(m, p, items, stream)
+                          : launch_attn_as<T, DP, NT, false>(m, p, items, stream);
 }
 
 template <typename T>
@@ -867,9 +986,9 @@ using namespace actune;
 extern "C" {
 
 size_t actune_prefix_attention_workspace_size(int64_t B, int64_t T, int64_t H, int64_t KV, int64_t D, int64_t G,
-                                              int64_t P, int64_t S) {
+                                              int64_t P, int64_t S, int ragged) {
   if (!attn_sizes_ok(B, T, H, KV, D, G, P, S) || B == 0 || T == 0) return 0;
-  return attn_workspace(attn_plan(B, T, H, KV, D, G, P, S), B * T * H, D);
+  return attn_workspace(attn_plan(B, T, H, KV, D, G, P, S, ragged != 0), B * T * H, D);
 }
 
 int actune_prefix_attention(const actune_prefix_attention_args* a, void* stream) {
@@ -890,7 +1009,7 @@ int actune_prefix_attention(const actune_prefix_attention_args* a, void* stream)
     if (!is_aligned(x, 2)) return ACTUNE_ERR_MISALIGNED;
   for (const void* x : {a->starts, a->prefix_lens, a->lens})
     if (!is_aligned(x, 4)) return ACTUNE_ERR_MISALIGNED;
-  const AttnPlan c = attn_plan(a->B, a->T, a->H, a->KV, a->D, a->G, a->P, a->S);
+  const AttnPlan c = attn_plan(a->B, a->T, a->H, a->KV, a->D, a->G, a->P, a->S, a->starts != nullptr);
   const int64_t rows = a->B * a->T * a->H;
   const size_t need = attn_workspace(c, rows, a->D);
   if (need > 0 && (a->workspace == nullptr || a->workspace_bytes < need)) return ACTUNE_ERR_WORKSPACE;
@@ -925,7 +1044,7 @@ int actune_prefix_attention(const actune_prefix_attention_args* a, void* stream)
                               ? launch_pdl(prefix_attention_any_kernel<__nv_bfloat16>, grid, 128, 0, cs, p)
                               : launch_pdl(prefix_attention_any_kernel<__half>, grid, 128, 0, cs, p));
   }
-  p.tiles_per_seq = c.tiles_per_seq, p.stacked = c.stacked, p.prefix_tiles = c.prefix_tiles;
+  p.tiles_per_seq = c.tiles_per_seq, p.kind = c.kind, p.prefix_tiles = c.prefix_tiles;
   p.prefix_splits = c.prefix_splits, p.own_splits = c.own_splits, p.splits = c.splits;
   p.ml = reinterpret_cast<float2*>(reinterpret_cast<uint8_t*>(a->workspace) + (size_t)c.splits * rows * p.D * 4);
   p.o_part = reinterpret_cast<float*>(a->workspace);

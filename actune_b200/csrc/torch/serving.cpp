@@ -270,7 +270,7 @@ PyObject* shared_prefix_attention(PyObject* const* a) {
             "out must be contiguous and match q");
   else
     out = empty(q.sizes(), dtype, device);
-  g.workspace_bytes = actune_prefix_attention_workspace_size(g.B, g.T, g.H, g.KV, g.D, g.G, g.P, g.S);
+  g.workspace_bytes = actune_prefix_attention_workspace_size(g.B, g.T, g.H, g.KV, g.D, g.G, g.P, g.S, g.starts != nullptr);
   Tensor workspace;
   if (g.workspace_bytes > 0) {
     workspace = empty({(int64_t)g.workspace_bytes}, at::kByte, device);

@@ -133,8 +133,9 @@ typedef struct actune_prefix_attention_args {
   int32_t dtype, causal;
 } actune_prefix_attention_args;
 
+/* ragged: whether starts will be given. */
 size_t actune_prefix_attention_workspace_size(int64_t B, int64_t T, int64_t H, int64_t KV, int64_t D, int64_t G,
-                                              int64_t P, int64_t S);
+                                              int64_t P, int64_t S, int ragged);
 int actune_prefix_attention(const actune_prefix_attention_args* args, void* stream);
 
 #ifdef __cplusplus

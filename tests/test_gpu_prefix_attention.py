@@ -116,6 +116,37 @@ def test_ragged_groups_and_lengths_over_stale_memory(D, T, causal):
     assert not out[10].any()
 
 
+# Tiles that hold rows of several sequences and their own keys too (chosen when there are
+# tiles enough): 40 and 33 rows a sequence against tiles of 128 and 256.
+@pytest.mark.parametrize("causal", [False, True])
+@pytest.mark.parametrize("D,T,H,KV", [(256, 5, 8, 1), (256, 50, 8, 1), (128, 10, 16, 4), (64, 33, 8, 8), (72, 11, 6, 2)])
+def test_tiles_across_sequences(D, T, H, KV, causal):
+    from actune_b200 import _lib
+    B, G, P, S = 120, 3, 260, 90
+    assert _lib.lib().actune_prefix_attention_workspace_size(B, T, H, KV, D, G, P, S, 1) == 0  # nothing to join
+    q, pk, pv, k, v = operands(B, T, H, KV, D, G, P, S, torch.bfloat16, T)
+    starts, plens = [0, 61, 61, 120], [259, 5, 130]
+    lens = [(7 * b) % (S + 1) for b in range(B)]  # from zero on
+    for t, lengths in ((pk, plens), (pv, plens), (k, lens), (v, lens)):
+        for i, n in enumerate(lengths):
+            t[i, n:] = float("nan") if i % 2 else float("inf")
+    run_and_check(q, pk, pv, k, v, starts=starts, plens=plens, lens=lens, causal=causal)
+    run_and_check(q, pk, pv, k, v, starts=starts, plens=[0, 0, 0], lens=lens, causal=causal)
+
+
+@pytest.mark.parametrize("D,H,KV", [(256, 8, 1), (128, 8, 2)])
+def test_one_request_does_not_reach_another_in_its_tile(D, H, KV):
+    from actune_b200 import ops
+    q, pk, pv, k, v = operands(100, 9, H, KV, D, 2, 200, 70, torch.bfloat16, 9)
+    clean = ops.shared_prefix_attention(q, pk, pv, k, v)
+    bad = [3, 4, 17, 51]
+    v[3], k[4, 2], v[17, 69], q[51] = float("inf"), float("nan"), float("nan"), float("nan")
+    dirty = ops.shared_prefix_attention(q, pk, pv, k, v)
+    keep = [b for b in range(100) if b not in bad]
+    assert torch.equal(clean[keep], dirty[keep])
+    assert all(not dirty[b].isfinite().any() for b in bad)
+
+
 def test_rows_that_see_nothing_are_zero():
     q, pk, pv, k, v = operands(3, 6, 4, 2, 64, 1, 16, 10, torch.bfloat16, 1)
     out = run_and_check(q, pk, pv, k, v, plens=[0], lens=[2, 6, 10], causal=True)
