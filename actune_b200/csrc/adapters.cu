@@ -13,6 +13,11 @@
 // its fragment registers.  v enters the second product as the sum of two 16-bit parts
 // (v = hi + lo, 16 bits of significand or more), so it keeps its 32-bit precision up to
 // the accumulator for twice a small number of MMAs.
+//
+// The expand kernel has three forms: 4-row tiles without the matrix units (their time is
+// latency: `up` asked for before v is there), 16 and 32 rows by mma.sync, and 128 rows on
+// tcgen05 with y and out as boxes by TMA (their time is that traffic).  16 requests of 304
+// tokens, 2048 -> 32768, rank 64: @VLM@, the floor of its bytes 114 us.
 #include "serving.cuh"
 
 namespace actune {

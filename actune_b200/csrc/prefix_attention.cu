@@ -7,30 +7,39 @@
 //   m' = max(m, max s),  p = 2^(s - m'),  l' = l 2^(m - m') + sum p,  O' = O 2^(m - m') + p V
 // (s in units of log2).  Parts of the keys computed apart are joined by the same rule.
 //
-// A work item is a tile of 128 (or 2 x 128) query rows of one key/value head and a range
-// of 128 keys (64 at head sizes above 128) at a time.  There are three ways to make tiles:
+// A work item is a tile of 128 query rows (or 2 of 128, where head size and rows allow) of
+// one key/value head, and a range of keys, 64 at a time.  There are three ways to make tiles:
 //   * by sequence: the rows (token, query head of the group) of one sequence against its
-//     prefix and then its own keys.  One launch when there are tiles enough.
+//     prefix and then its own keys.
 //   * stacked: for the prefix, the rows of all sequences that share it are stacked, so a
 //     prefix is read once for the batch and not once per sequence; each sequence's own
 //     keys are a further item, and the parts are joined by a second kernel.  For few
-//     query rows, whose own keys need the tiles' rows for little.
+//     query rows, whose own keys need the tiles' rows for little: 32 single tokens behind
+//     4 x 4096, 8 heads on one of 256: 50 us, 148 us by sequence.
 //   * mixed: stacked tiles that go through the prefix and then through the own keys of
 //     each of their sequences, the product with V writing that sequence's rows alone.
-//     For tiles of few sequences, when there are tiles enough: no parts to join.
+//     For tiles of few sequences, when there are tiles enough: no parts to join.  16
+//     prefixes of 304 x 8 sequences of 50 tokens: 39 us, 46 us by sequence.
 // In the first two the key range is split over more items when tiles are few.  No value
 // of one request enters another's sums, not even multiplied by zero.
 //
 // One item per CTA:
-//   softmax warps   4 per 128 rows, thread = row: scores from tensor memory to registers,
-//                   mask, maximum, exponentials, sum; p (16 bit) back to tensor memory
-//   one warp        TMA producer: K and V blocks into a ring of 128-byte-swizzled tiles
-//   one warp        tcgen05.mma issuer: S = Q K^T (both operands in shared memory),
+//   softmax warps   8 per 128 rows, two threads a row (32 keys of a block each): scores from
+//                   tensor memory to registers, mask, maximum, exponentials, sum; p (16
+//                   bit) back to tensor memory
+//   one warp        TMA producer: a ring of 128-byte-swizzled tiles, a stage holding K of
+//                   one block and V of the one two before it, the two used together
+//   one warp a tile tcgen05.mma issuer: S = Q K^T (both operands in shared memory),
 //                   O += P V (P in tensor memory, V as the MN-major operand)
-// S of the next block is computed while this block's softmax runs (two score buffers
-// for one row tile, the other row tile's scores for two).  O is rescaled only when the
-// maximum has grown by more than 2^8 since the last time: until then p stays below 2^8,
-// which the 16-bit types and the fp32 sums hold, and l and O carry the same factor.
+// S of the next block is computed while this block's softmax runs (two score buffers a
+// row tile).  O is rescaled only when the maximum has grown by more than 2^8 since the
+// last time: until then p stays below 2^8, which the 16-bit types and the fp32 sums hold,
+// and l and O carry the same factor.
+//
+// Bounds: at head sizes up to 128 a block of 64 keys asks 128 rows x 64 exponentials of
+// each tile, as long as its products; with the softmax's latency between the two products
+// the main loop holds 65-70% of the measured matrix rate (75% at 256).  16 x 56 tokens, 32
+// heads of 128 behind 2 histories of up to 8192: @OFT@.  Small calls are launch, prologue and join.
 #include "serving.cuh"
 
 namespace actune {
@@ -80,7 +89,7 @@ struct AttnParams {
   int prefix_splits, own_splits;  // by sequence: prefix_splits of both together
   int splits;       // parts per row; 1: write out directly
   int q_boxes;      // query tiles come by tensor map (tokens evenly spaced, rep a divisor of 128)
-  Divisor by_prefix_tiles, by_kv, by_own_tiles, by_tiles_per_seq, by_per_seq, by_rep, by_prefix_splits, by_own_splits;
+  Divisor by_full_tiles, by_prefixes, by_kv, by_own_tiles, by_tiles_per_seq, by_per_seq, by_rep, by_prefix_splits, by_own_splits;
 };
 
 __device__ __forceinline__ int clamp_len(const int32_t* lens, int i, int most) {
@@ -271,6 +280,8 @@ __device__ AttnItem attn_item(const AttnParams& p, int lane, TileSeqs& seqs) {
   AttnItem it = {};
   const int per_seq = p.T * p.rep;
   int x = blockIdx.x;
+  // Full tiles first: the last one of each prefix may have few rows, and fills the gaps.
+  const int full_items = p.kind != kBySequence ? (p.prefix_tiles - p.G) * p.KV * p.prefix_splits : 0;
   const int prefix_items = p.kind != kBySequence ? p.prefix_tiles * p.KV * p.prefix_splits : 0;
   // Part `i` of `blocks` blocks dealt to d.d parts: [begin, end).
   const auto deal = [](int blocks, const Divisor& d, int i, int& begin, int& end) {
@@ -280,7 +291,9 @@ __device__ AttnItem attn_item(const AttnParams& p, int lane, TileSeqs& seqs) {
     end = begin + each + (i < more);
   };
   if (x < prefix_items) {
-    const int tile = p.by_prefix_tiles.split(x);
+    const bool full = x < full_items;
+    if (!full) x -= full_items;
+    const int tile = full ? p.by_full_tiles.split(x) : p.by_prefixes.split(x);
     it.kv = p.by_kv.split(x), it.split = x;
     // The prefix whose stacked rows hold this tile: running count of tiles, 32 prefixes a step.
     int before = 0;
@@ -297,7 +310,7 @@ __device__ AttnItem attn_item(const AttnParams& p, int lane, TileSeqs& seqs) {
           s1 = (int)(((int64_t)(g + 1) * p.B + p.G - 1) / p.G);
         }
       }
-      const int rows = (s1 - s0) * per_seq, mine = (rows + ROWS - 1) / ROWS;
+      const int rows = (s1 - s0) * per_seq, mine = full ? rows / ROWS : rows % ROWS != 0;
       int upto = mine;
 #pragma unroll
       for (int o = 1; o < 32; o <<= 1) {
@@ -310,8 +323,9 @@ __device__ AttnItem attn_item(const AttnParams& p, int lane, TileSeqs& seqs) {
         const int first = before + upto - mine;
         it.g = base + src;
         it.seq0 = __shfl_sync(0xffffffffu, s0, src);
-        it.row0 = (tile - __shfl_sync(0xffffffffu, first, src)) * ROWS;
-        it.nrows = min(ROWS, __shfl_sync(0xffffffffu, rows, src) - it.row0);
+        const int all = __shfl_sync(0xffffffffu, rows, src);
+        it.row0 = full ? (tile - __shfl_sync(0xffffffffu, first, src)) * ROWS : all / ROWS * ROWS;
+        it.nrows = min(ROWS, all - it.row0);
         found = true;
       }
       before += __shfl_sync(0xffffffffu, upto, 31);
@@ -495,6 +509,7 @@ __global__ void __launch_bounds__(AttnCfg<DP, NT>::WARPS * 32, 1)
     // increment of the one before: address arithmetic between two MMAs is time the tensor
     // core waits.
     const int t = warp - kIssuer;
+    const bool used = t * 128 < it.nrows;  // a tile without rows goes through the steps alone
     if (nblk > 0 && lane == 0) {
       const uint64_t q_desc = smem_desc_sw128(smem_u32(smem) + t * (128 * DP * 2));
       const uint64_t k_desc0 = smem_desc_sw128(smem_u32(ring)), v_desc0 = smem_desc_mn_sw128(smem_u32(ring) + C::SLOT_BYTES, BN);
@@ -523,7 +538,7 @@ __global__ void __launch_bounds__(AttnCfg<DP, NT>::WARPS * 32, 1)
              (i < 0 || mbar_wait(&p_ready[t][buffer], turn, kSiteAttn + 3));
         if (!ok) break;
         tc_fence_after();
-        if (i >= 0) {
+        if (i >= 0 && used) {
           const uint64_t v_desc = v_desc0 + (uint32_t)slot * kStageStep;
           // Each half of the keys has its p over its own scores.
           const auto p_at = [&](int k) { return s_at + (k / (BN / 32)) * (BN / 2) + (k % (BN / 32)) * 8; };
@@ -539,8 +554,9 @@ __global__ void __launch_bounds__(AttnCfg<DP, NT>::WARPS * 32, 1)
               const uint32_t upto = hi <= 0 ? 0u : hi >= 32 ? ~0u : (1u << hi) - 1u;
               off[w] = ~(upto & ~below);
             }
+            const bool any = (off[0] & off[1] & off[2] & off[3]) != ~0u;
 #pragma unroll
-            for (int k = 0; k < BN / 16; ++k)
+            for (int k = 0; k < BN / 16 && any; ++k)
               mma16_ts_rows(o_col, p_at(k), v_desc + k * (2048 / 16), idesc_16<T>(DP, true), add || k > 0, off);
           } else {
 #pragma unroll
@@ -548,7 +564,7 @@ __global__ void __launch_bounds__(AttnCfg<DP, NT>::WARPS * 32, 1)
               mma16_ts(o_col, p_at(k), v_desc + k * (2048 / 16), idesc_16<T>(DP, true), i > 0 || k > 0);
           }
         }
-        if (i + NB < nblk) scores(s_at);
+        if (i + NB < nblk && used) scores(s_at);
         mma_commit(&step[t][buffer]);
         mma_commit(&empty[slot]);
         next();
@@ -878,8 +894,12 @@ AttnPlan attn_plan(int64_t B, int64_t T, int64_t H, int64_t KV, int64_t D, int64
     c.tiles_per_seq = (int)ceil_div(per_seq, tile);
     c.prefix_tiles = kind != kBySequence ? (int)(B * per_seq / tile + G) : 0;
     const int64_t own_tiles = B * c.tiles_per_seq * KV;
-    // Uneven groups leave up to a part of a tile each.
-    const int64_t tiles = (ragged ? c.prefix_tiles : G * ceil_div(ceil_div(B, G) * per_seq, tile)) * KV;
+    // Full tiles of a stack, and the last ones of the prefixes, which uneven groups leave
+    // with any number of rows: of two row tiles the second is often empty, and skipped.
+    const int64_t stack = ceil_div(B, G) * per_seq;
+    const int64_t full = ragged ? B * per_seq / tile : G * (stack / tile);
+    const int64_t last = ragged ? G : stack % tile > 0 ? G : 0;
+    const int64_t last_block = nt == 1 ? block : ragged ? 7 : stack % tile > 128 ? 9 : 6;
     const auto waves = [&](int64_t items, int64_t blocks) {
       return ceil_div(items, kSmsPlanned) * (blocks * block + kStart);
     };
@@ -895,14 +915,15 @@ AttnPlan attn_plan(int64_t B, int64_t T, int64_t H, int64_t KV, int64_t D, int64
       // Blocks per item that fill one wave, prefix and own keys together.  (More parts than
       // that measured slower: 8 single tokens behind 4096, 22 us with 10 + 2 parts, 30 us
       // with 18 + 1.)
-      const int64_t even = ceil_div(B * per_seq, tile) * KV;
-      int64_t each = ceil_div(even * pb + own_tiles * ob, kSmsPlanned);
+      int64_t each = ceil_div(ceil_div(B * per_seq, tile) * KV * pb + own_tiles * ob, kSmsPlanned);
       each = each < 2 ? 2 : each;
       int64_t n = ceil_div(pb, each), os = S > 0 ? ceil_div(ob, each) : 0;
       n = n > kMost ? kMost : n, os = os > 16 ? 16 : os;
       c.prefix_splits = (int)n;
-      cost = (even * n * (ceil_div(pb, n) * block + kStart) +
-              (os > 0 ? own_tiles * os * (ceil_div(ob, os) * block + kStart) : 0)) / kSmsPlanned + kStart + join(n + os);
+      const int64_t part = ceil_div(pb, n);
+      cost = (KV * n * (full * (part * block + kStart) + last * (part * last_block + kStart)) +
+              (os > 0 ? own_tiles * os * (ceil_div(ob, os) * block + kStart) : 0)) / kSmsPlanned +
+             (part * block + kStart) / 2 + join(n + os);
       c.own_splits = (int)os;
       c.splits = (int)(c.prefix_splits + os);
       c.items = (int64_t)c.prefix_tiles * KV * c.prefix_splits + own_tiles * os;
@@ -911,7 +932,15 @@ AttnPlan attn_plan(int64_t B, int64_t T, int64_t H, int64_t KV, int64_t D, int64
       if (touched > kMixedSeqs) continue;
       c.prefix_splits = c.splits = 1;
       c.items = (int64_t)c.prefix_tiles * KV;
-      cost = waves(tiles, pb + (tile / per_seq + 1) * ob);
+      // The full tiles come first, and the last of each prefix fill what they leave free.
+      const int64_t own = (tile / per_seq + 1) * ob;
+      const int64_t t = (pb + own) * block + kStart, t_last = (pb + own) * last_block + kStart;
+      const int64_t n = full * KV, n_last = last * KV, free = ceil_div(n, kSmsPlanned) * kSmsPlanned - n;
+      cost = ceil_div(n, kSmsPlanned) * t;
+      if (n_last > free) {
+        const int64_t all = (n * t + n_last * t_last) / kSmsPlanned + t_last / 2;
+        cost = cost > all ? cost : all;
+      }
     }
     if (cost < best_cost) best_cost = cost, best = c;
   }
@@ -1048,7 +1077,7 @@ int actune_prefix_attention(const actune_prefix_attention_args* a, void* stream)
   p.prefix_splits = c.prefix_splits, p.own_splits = c.own_splits, p.splits = c.splits;
   p.ml = reinterpret_cast<float2*>(reinterpret_cast<uint8_t*>(a->workspace) + (size_t)c.splits * rows * p.D * 4);
   p.o_part = reinterpret_cast<float*>(a->workspace);
-  p.by_prefix_tiles.set(c.prefix_tiles > 0 ? c.prefix_tiles : 1), p.by_kv.set(p.KV);
+  p.by_full_tiles.set(c.prefix_tiles > p.G ? c.prefix_tiles - p.G : 1), p.by_prefixes.set(p.G), p.by_kv.set(p.KV);
   p.by_own_tiles.set((int64_t)p.B * c.tiles_per_seq), p.by_tiles_per_seq.set(c.tiles_per_seq);
   p.by_per_seq.set((int64_t)p.T * p.rep), p.by_rep.set(p.rep);
   p.by_prefix_splits.set(c.prefix_splits > 0 ? c.prefix_splits : 1), p.by_own_splits.set(c.own_splits > 0 ? c.own_splits : 1);
