@@ -1,7 +1,7 @@
 // Low-rank adapters of many requests beside a shared projection (sm_100a):
 //   out[m] = y[m] + scale[s] * up[s] (down[s] x[m]),   s = slots[m].
 //
-// plan    rows sorted by adapter into tiles of 4, 16, 32 or 128 rows with one adapter each.
+// plan    rows sorted by adapter into tiles of 4, 16 or 128 rows with one adapter each.
 // shrink  v = down x for a tile and a slice of K; the slices' fp32 sums go to the
 //         workspace, so that few rows still occupy the machine, in a fixed order.
 // expand  out = y + scale * up v for a tile and a range of columns.
@@ -15,7 +15,7 @@
 // the accumulator for twice a small number of MMAs.
 //
 // The expand kernel has three forms: 4-row tiles without the matrix units (their time is
-// latency: `up` asked for before v is there), 16 and 32 rows by mma.sync, and 128 rows on
+// latency: `up` asked for before v is there), 16 rows by mma.sync, and 128 rows on
 // tcgen05 with y and out as boxes by TMA (their time is that traffic).  16 requests of 304
 // tokens, 2048 -> 32768, rank 64: @VLM@, the floor of its bytes 114 us.
 #include "serving.cuh"
@@ -569,7 +569,9 @@ __global__ void __launch_bounds__(ExpandCfg<RP>::THREADS, 1)
     int boxes = 0;
 #pragma unroll
     for (int q = 0; q < 4; ++q) {
-      at[q] = steps > 0 && boxed(q) ? order[32 * q] : -1;
+      // A box may bring rows behind the tile's, which count for nothing, but not many.
+      const int n = min(32, tile.z - 32 * q);
+      at[q] = steps > 0 && p.boxes && n >= 16 && order[32 * q + n - 1] - order[32 * q] == n - 1 ? order[32 * q] : -1;
       boxes += at[q] >= 0;
       const int r = 32 * q + lane;
       rows[q] = steps > 0 && at[q] < 0 && r < tile.z ? reinterpret_cast<const T*>(p.y) + order[r] * p.y_stride : nullptr;
@@ -749,6 +751,20 @@ int steps_per_cta(int64_t spans, const AdapterParams& p, int tile, int most) {
   return (int)(steps < 1 ? 1 : steps > most ? most : steps);
 }
 
+// The same where an SM holds one CTA: the steps that end first, a CTA's start and end
+// taken for two of them.  Up to 16, so that tiles of few rows and of many even out (40 x
+// 150 rows 1024 -> 8192: 82 us, 106 us with 64).
+int steps_of_one_per_sm(int64_t spans, const AdapterParams& p, int tile) {
+  const int64_t tiles = ceil_div(p.M, tile) + (p.S < p.M ? p.S : p.M) / 2;
+  int64_t best = INT64_MAX;
+  int steps = 1;
+  for (int n = 1; n <= 16; ++n) {
+    const int64_t cost = ceil_div(tiles * ceil_div(spans, n), kSmsPlanned) * (n + 2);
+    if (cost < best) best = cost, steps = n;
+  }
+  return steps;
+}
+
 template <typename T, int TILE, int RP, bool VEC>
 cudaError_t launch_adapter(AdapterParams p, const CUtensorMap* maps, cudaStream_t stream) {
   if constexpr (TILE == 128 && VEC) {
@@ -761,10 +777,8 @@ cudaError_t launch_adapter(AdapterParams p, const CUtensorMap* maps, cudaStream_
       if (e != cudaSuccess) return e;
       e = ensure_smem_limit<adapter_expand128_kernel<T, RP>>(C::SMEM);
       if (e != cudaSuccess) return e;
-      // One CTA per SM; up to 16 steps a CTA, so that tiles of few rows and of many even out
-      // (40 x 150 rows 1024 -> 8192: 82 us, 106 us with 64 steps).
       const int64_t spans = ceil_div(p.N, 128);
-      p.col_steps = steps_per_cta(2 * spans, p, TILE, 16);
+      p.col_steps = steps_of_one_per_sm(spans, p, TILE);
       return launch_pdl(adapter_expand128_kernel<T, RP>, dim3((unsigned)ceil_div(spans, p.col_steps), p.tiles_cap),
                         C::THREADS, C::SMEM, stream, maps[0], maps[1], maps[2], maps[3], p);
     }
@@ -781,9 +795,7 @@ cudaError_t launch_adapter(AdapterParams p, const CUtensorMap* maps, cudaStream_
                         stream, p);
     }
   }
-  // Two 16-row blocks per warp halve the reads of `up`; at rank 128 the split v of one
-  // block already takes 64 registers.
-  constexpr int MW = TILE == 128 || (TILE >= 32 && RP <= 64) ? 2 : 1;
+  constexpr int MW = TILE == 128 ? 2 : 1;  // two 16-row blocks per warp halve the reads of `up`
   constexpr int EWM = WM / MW;
   const int64_t spans = ceil_div(p.N, 64 * (4 / EWM));
   p.col_steps = steps_per_cta(spans, p, TILE, 8);
@@ -804,8 +816,6 @@ cudaError_t dispatch(const AdapterParams& p, const CUtensorMap* maps, int tile, 
     ACTUNE_ADAPTER(kFewRows)
   } else if (tile == 16) {
     ACTUNE_ADAPTER(16)
-  } else if (tile == 32) {
-    ACTUNE_ADAPTER(32)
   }
   ACTUNE_ADAPTER(128)
 #undef ACTUNE_ADAPTER
@@ -836,7 +846,7 @@ int encode_matrix(CUtensorMap* map, int dtype, const void* base, int64_t rows, i
 }
 
 bool valid_plan(int64_t M, int64_t S, int tile) {
-  return M >= 0 && M <= (1 << 28) && S > 0 && S <= kMaxSlots && (tile == kFewRows || tile == 16 || tile == 32 || tile == 128) &&
+  return M >= 0 && M <= (1 << 28) && S > 0 && S <= kMaxSlots && (tile == kFewRows || tile == 16 || tile == 128) &&
          max_tiles(M, S, tile) <= 65535;
 }
 

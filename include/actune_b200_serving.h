@@ -58,7 +58,7 @@ int actune_gated_norm(const actune_gated_norm_args* args, void* stream);
  * for y the shared projection's output; rows whose slot is outside 0 .. S-1 keep y[m].
  *
  * actune_adapter_plan sorts the rows of a batch by slot (stable) into tiles of `tile`
- * rows (4, 16, 32 or 128) that share one adapter; every projection and layer the batch
+ * rows (4, 16 or 128) that share one adapter; every projection and layer the batch
  * passes through reads the same plan.  slots: int32 [M] on the device, so a captured
  * graph can follow a batch whose routing changes.  plan: int32 buffer of
  * actune_adapter_plan_size(M, S, tile) bytes, 16-byte aligned.  S <= 8191.
