@@ -16,7 +16,8 @@
 //
 // The expand kernel has three forms: 4-row tiles without the matrix units (their time is
 // latency: `up` asked for before v is there), 16 rows by mma.sync, and 128 rows on
-// tcgen05 with y and out as boxes by TMA (their time is that traffic).  16 requests of 304
+// tcgen05 with y and out as boxes by TMA (their time is that traffic; with little of it
+// tiles of 128 take the 16-row form in parts).  16 requests of 304
 // tokens, 2048 -> 32768, rank 64: @VLM@, the floor of its bytes 114 us.
 #include "serving.cuh"
 
@@ -175,79 +176,73 @@ __device__ __forceinline__ void split2(float a, float b, uint32_t& hi, uint32_t&
   lo = *reinterpret_cast<const uint32_t*>(&parts[2]);
 }
 
-// v = down x for WM * 16 rows of a tile.  WM warps side by side along the rows (16 each)
-// and WK along K; a warp's K steps are 32 elements: lane (g, t) holds elements 8t .. 8t + 7
-// of rows g and g + 8 of x and of row g of each 8-row block of down, two MMAs per block.
-// Nothing is shared between warps until their sums are added in shared memory.
+// v = down x for 16 rows of a tile (a tile of 128 takes eight CTAs, blockIdx.z).  The warps
+// share K; a warp's steps are 32 elements: lane (g, t) holds elements 8t .. 8t + 7 of rows g
+// and g + 8 of x and of row g of each 8-row block of down, two MMAs per block.  Nothing is
+// shared between warps until their sums are added in shared memory.
 //
-// SPLIT: 16 rows of a 128-row tile and all of K, 8 warps; the sums are complete, and go
-// out as the two 16-bit parts that the next kernel takes.  Else a tile and one slice of K;
-// the slice's sums go out in fp32.
-constexpr int shrink_warps(int wm, bool split) { return split || wm > 4 ? 8 : 4; }
-constexpr int shrink_shared(int wm, int rp, bool split) { return (shrink_warps(wm, split) / wm - 1) * wm * 16 * rp * 4; }
+// SPLIT: all of K, 8 warps; the sums are complete, and go out as the two 16-bit parts that
+// the tcgen05 form takes.  Else one slice of K, 4 warps; its sums go out in fp32.
+constexpr int shrink_warps(bool split) { return split ? 8 : 4; }
+constexpr int shrink_shared(int rp, bool split) { return (shrink_warps(split) - 1) * 16 * rp * 4; }
 
-template <typename T, int WM, int RP, bool VEC, bool SPLIT>
-__global__ void __launch_bounds__(32 * shrink_warps(WM, SPLIT)) adapter_shrink_kernel(const AdapterParams p) {
-  constexpr int WK = shrink_warps(WM, SPLIT) / WM, NT = RP / 8;
-  extern __shared__ float part[];  // [WK - 1, WM, 16 * RP]
+template <typename T, int RP, bool VEC, bool SPLIT>
+__global__ void __launch_bounds__(32 * shrink_warps(SPLIT)) adapter_shrink_kernel(const AdapterParams p) {
+  constexpr int WK = shrink_warps(SPLIT), NT = RP / 8;
+  extern __shared__ float part[];  // [WK - 1, 16 * RP]
   griddep_enter();
   if ((int)blockIdx.x >= p.plan[0]) return;
   int4 tile = plan_tiles(p.plan)[blockIdx.x];
-  if constexpr (SPLIT) tile.y += blockIdx.y * (WM * 16), tile.z -= blockIdx.y * (WM * 16);
+  tile.y += blockIdx.z * 16, tile.z -= blockIdx.z * 16;
   if (tile.x < 0 || tile.z <= 0) return;
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int lane = threadIdx.x & 31, wk = threadIdx.x >> 5;
   const int g = lane >> 2, t = lane & 3;
-  const int wm = warp % WM, wk = warp / WM;
   const int32_t* order = plan_rows(p) + tile.y;
   const T* rows[2];
 #pragma unroll
   for (int h = 0; h < 2; ++h) {
-    const int i = wm * 16 + g + 8 * h;
+    const int i = g + 8 * h;
     rows[h] = i < tile.z ? reinterpret_cast<const T*>(p.x) + order[i] * p.x_stride : nullptr;
   }
   const T* down = reinterpret_cast<const T*>(p.down) + (int64_t)tile.x * p.R * p.K;
   const int k0 = SPLIT ? 0 : blockIdx.y * p.k_slice, k1 = SPLIT ? p.K : min(p.K, k0 + p.k_slice);
   float acc[NT][4] = {};
-  if (wm * 16 < tile.z) {
-    constexpr int UNROLL = RP <= 64 ? 4 : 2;  // steps whose loads go out together
+  constexpr int UNROLL = RP <= 64 ? 4 : 2;  // steps whose loads go out together
 #pragma unroll UNROLL
-    for (int k = k0 + wk * 32; k < k1; k += WK * 32) {
-      const int e = k + 8 * t;
-      uint32_t xa[2][4], db[NT][4];
+  for (int k = k0 + wk * 32; k < k1; k += WK * 32) {
+    const int e = k + 8 * t;
+    uint32_t xa[2][4], db[NT][4];
 #pragma unroll
-      for (int h = 0; h < 2; ++h) load_run<T, VEC, 8>(xa[h], rows[h], e, rows[h] ? k1 : 0);
+    for (int h = 0; h < 2; ++h) load_run<T, VEC, 8>(xa[h], rows[h], e, rows[h] ? k1 : 0);
 #pragma unroll
-      for (int j = 0; j < NT; ++j)
-        load_run<T, VEC, 8>(db[j], down + (int64_t)(j * 8 + g) * p.K, e, j * 8 + g < p.R ? k1 : 0);
+    for (int j = 0; j < NT; ++j)
+      load_run<T, VEC, 8>(db[j], down + (int64_t)(j * 8 + g) * p.K, e, j * 8 + g < p.R ? k1 : 0);
 #pragma unroll
-      for (int j = 0; j < NT; ++j) {
-        const uint32_t a0[4] = {xa[0][0], xa[1][0], xa[0][1], xa[1][1]};
-        const uint32_t a1[4] = {xa[0][2], xa[1][2], xa[0][3], xa[1][3]};
-        mma16816<T>(acc[j], a0, db[j][0], db[j][1]);
-        mma16816<T>(acc[j], a1, db[j][2], db[j][3]);
-      }
+    for (int j = 0; j < NT; ++j) {
+      const uint32_t a0[4] = {xa[0][0], xa[1][0], xa[0][1], xa[1][1]};
+      const uint32_t a1[4] = {xa[0][2], xa[1][2], xa[0][3], xa[1][3]};
+      mma16816<T>(acc[j], a0, db[j][0], db[j][1]);
+      mma16816<T>(acc[j], a1, db[j][2], db[j][3]);
     }
   }
-  if constexpr (WK > 1) {
-    if (wk > 0) {
-      float* mine = part + ((wk - 1) * WM + wm) * 16 * RP;
+  if (wk > 0) {
+    float* mine = part + (wk - 1) * 16 * RP;
 #pragma unroll
-      for (int j = 0; j < NT; ++j)
+    for (int j = 0; j < NT; ++j)
 #pragma unroll
-        for (int e = 0; e < 4; ++e) mine[(j * 4 + e) * 32 + lane] = acc[j][e];
-    }
-    __syncthreads();
-    if (wk > 0) return;
-#pragma unroll
-    for (int w = 0; w < WK - 1; ++w)
-#pragma unroll
-      for (int j = 0; j < NT; ++j)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) acc[j][e] += part[(w * WM + wm) * 16 * RP + (j * 4 + e) * 32 + lane];
+      for (int e = 0; e < 4; ++e) mine[(j * 4 + e) * 32 + lane] = acc[j][e];
   }
+  __syncthreads();
+  if (wk > 0) return;
+#pragma unroll
+  for (int w = 0; w < WK - 1; ++w)
+#pragma unroll
+    for (int j = 0; j < NT; ++j)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) acc[j][e] += part[w * 16 * RP + (j * 4 + e) * 32 + lane];
 #pragma unroll
   for (int h = 0; h < 2; ++h) {
-    const int i = wm * 16 + g + 8 * h;
+    const int i = g + 8 * h;
     if constexpr (SPLIT) {
       float down_by = 1.f, factor = p.scale[tile.x];
       if constexpr (std::is_same<T, __half>::value) {
@@ -353,89 +348,83 @@ __global__ void __launch_bounds__(128) adapter_expand_few_kernel(const AdapterPa
   }
 }
 
-// out = y + scale * up v.  A warp keeps the split v of MW * 16 rows in registers and
-// walks col_steps steps of 64 columns; the columns of a step are dealt so that lane
-// (g, t) ends up with columns 8t .. 8t + 7 and 32 + 8t .. 32 + 8t + 7 of rows g and g + 8:
-// a quad's 16-byte pieces of y and out lie side by side.
-template <typename T, int WM, int MW, int RP, bool VEC>
+// out = y + scale * up v.  A warp keeps the split v of 16 rows (a tile of 128 takes eight
+// CTAs, blockIdx.z) in registers and walks col_steps steps of 64 columns, four warps side by
+// side; the columns of a step are dealt so that lane (g, t) ends up with columns 8t .. 8t +
+// 7 and 32 + 8t .. 32 + 8t + 7 of rows g and g + 8: a quad's 16-byte pieces of y and out lie
+// side by side.
+template <typename T, int RP, bool VEC>
 __global__ void __launch_bounds__(128) adapter_expand_kernel(const AdapterParams p) {
-  constexpr int WN = 4 / WM, KS = RP / 16;
+  constexpr int KS = RP / 16;
   griddep_enter();
   if ((int)blockIdx.y >= p.plan[0]) return;
-  const int4 tile = plan_tiles(p.plan)[blockIdx.y];
-  if (tile.x < 0 && p.out == p.y) return;
+  int4 tile = plan_tiles(p.plan)[blockIdx.y];
+  tile.y += blockIdx.z * 16, tile.z -= blockIdx.z * 16;
+  if (tile.z <= 0 || (tile.x < 0 && p.out == p.y)) return;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int g = lane >> 2, t = lane & 3;
-  const int wm = warp % WM, wn = warp / WM;
-  const int first = wm * MW * 16;
-  if (first >= tile.z) return;
   const int32_t* order = plan_rows(p) + tile.y;
-  int64_t row[MW][2];
-  uint32_t hi[MW][KS][4], lo[MW][KS][4];
-  float factor[MW][2];
+  int64_t row[2];
+  uint32_t hi[KS][4], lo[KS][4];
+  float factor[2];
   const float scale = tile.x >= 0 ? p.scale[tile.x] : 0.f;
 #pragma unroll
-  for (int m = 0; m < MW; ++m) {
+  for (int h = 0; h < 2; ++h) {
+    const int i = g + 8 * h;
+    row[h] = i < tile.z ? order[i] : -1;
+    float4 v[KS];
+    float top = 0.f;
 #pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      const int i = first + m * 16 + g + 8 * h;
-      row[m][h] = i < tile.z ? order[i] : -1;
-      float4 v[KS];
-      float top = 0.f;
+    for (int k = 0; k < KS; ++k) v[k] = make_float4(0.f, 0.f, 0.f, 0.f);
+    if (i < tile.z && tile.x >= 0) {
+      const float* src = p.v + (int64_t)(tile.y + i) * RP + 4 * t;
+      constexpr int U = KS <= 2 ? 4 : 1;  // slices whose loads go out together
+      for (int s = 0; s < p.slices; s += U, src += U * (int64_t)p.M * RP) {
+        float4 a[U][KS];
 #pragma unroll
-      for (int k = 0; k < KS; ++k) v[k] = make_float4(0.f, 0.f, 0.f, 0.f);
-      if (i < tile.z && tile.x >= 0) {
-        const float* src = p.v + (int64_t)(tile.y + i) * RP + 4 * t;
-        constexpr int U = KS <= 2 ? 4 : 1;  // slices whose loads go out together
-        for (int s = 0; s < p.slices; s += U, src += U * (int64_t)p.M * RP) {
-          float4 a[U][KS];
+        for (int u = 0; u < U; ++u)
 #pragma unroll
-          for (int u = 0; u < U; ++u)
+          for (int k = 0; k < KS; ++k)
+            a[u][k] = s + u < p.slices ? *reinterpret_cast<const float4*>(src + u * (int64_t)p.M * RP + 16 * k)
+                                       : make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
-            for (int k = 0; k < KS; ++k)
-              a[u][k] = s + u < p.slices ? *reinterpret_cast<const float4*>(src + u * (int64_t)p.M * RP + 16 * k)
-                                         : make_float4(0.f, 0.f, 0.f, 0.f);
+        for (int u = 0; u < U; ++u)
 #pragma unroll
-          for (int u = 0; u < U; ++u)
-#pragma unroll
-            for (int k = 0; k < KS; ++k) v[k].x += a[u][k].x, v[k].y += a[u][k].y, v[k].z += a[u][k].z, v[k].w += a[u][k].w;
-        }
+          for (int k = 0; k < KS; ++k) v[k].x += a[u][k].x, v[k].y += a[u][k].y, v[k].z += a[u][k].z, v[k].w += a[u][k].w;
       }
-      factor[m][h] = scale;
-      if constexpr (std::is_same<T, __half>::value) {
+    }
+    factor[h] = scale;
+    if constexpr (std::is_same<T, __half>::value) {
 #pragma unroll
-        for (int k = 0; k < KS; ++k)
-          top = fmaxf(fmaxf(top, fmaxf(fabsf(v[k].x), fabsf(v[k].y))), fmaxf(fabsf(v[k].z), fabsf(v[k].w)));
-        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
-        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
-        float down;
-        factor[m][h] = scale * fp16_room(top, down);
+      for (int k = 0; k < KS; ++k)
+        top = fmaxf(fmaxf(top, fmaxf(fabsf(v[k].x), fabsf(v[k].y))), fmaxf(fabsf(v[k].z), fabsf(v[k].w)));
+      top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+      top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+      float down;
+      factor[h] = scale * fp16_room(top, down);
 #pragma unroll
-        for (int k = 0; k < KS; ++k) v[k].x *= down, v[k].y *= down, v[k].z *= down, v[k].w *= down;
-      }
+      for (int k = 0; k < KS; ++k) v[k].x *= down, v[k].y *= down, v[k].z *= down, v[k].w *= down;
+    }
 #pragma unroll
-      for (int k = 0; k < KS; ++k) {
-        split2<T>(v[k].x, v[k].y, hi[m][k][h], lo[m][k][h]);
-        split2<T>(v[k].z, v[k].w, hi[m][k][2 + h], lo[m][k][2 + h]);
-      }
+    for (int k = 0; k < KS; ++k) {
+      split2<T>(v[k].x, v[k].y, hi[k][h], lo[k][h]);
+      split2<T>(v[k].z, v[k].w, hi[k][2 + h], lo[k][2 + h]);
     }
   }
   const T* up = reinterpret_cast<const T*>(p.up) + (int64_t)max(tile.x, 0) * p.N * p.R;
-  const int span = WN * 64;
+  const int span = 4 * 64;
   for (int step = 0; step < p.col_steps; ++step) {
-    const int n0 = (blockIdx.x * p.col_steps + step) * span + wn * 64;
+    const int n0 = (blockIdx.x * p.col_steps + step) * span + warp * 64;
     if (n0 >= p.N) break;
     const int n = n0 + 8 * t;
-    uint32_t yv[MW][2][2][4];
+    uint32_t yv[2][2][4];
 #pragma unroll
-    for (int m = 0; m < MW; ++m)
+    for (int h = 0; h < 2; ++h)
 #pragma unroll
-      for (int h = 0; h < 2; ++h)
-#pragma unroll
-        for (int c = 0; c < 2; ++c)
-          load_run<T, VEC, 8>(yv[m][h][c], reinterpret_cast<const T*>(p.y) + row[m][h] * p.y_stride, n + 32 * c,
-                              row[m][h] >= 0 ? p.N : 0);
-    float acc[MW][8][4] = {};
+      for (int c = 0; c < 2; ++c)
+        load_run<T, VEC, 8>(yv[h][c], reinterpret_cast<const T*>(p.y) + row[h] * p.y_stride, n + 32 * c,
+                            row[h] >= 0 ? p.N : 0);
+    float acc[8][4] = {};
     if (tile.x >= 0) {
 #pragma unroll
       for (int k = 0; k < KS; ++k) {
@@ -444,38 +433,33 @@ __global__ void __launch_bounds__(128) adapter_expand_kernel(const AdapterParams
           const int col = n0 + 32 * (j >> 2) + 8 * (g >> 1) + 2 * (j & 3) + (g & 1);
           uint32_t b[2];
           load_run<T, VEC, 4>(b, up + (int64_t)col * p.R, 16 * k + 4 * t, col < p.N ? p.R : 0);
-#pragma unroll
-          for (int m = 0; m < MW; ++m) {
-            mma16816<T>(acc[m][j], hi[m][k], b[0], b[1]);
-            mma16816<T>(acc[m][j], lo[m][k], b[0], b[1]);
-          }
+          mma16816<T>(acc[j], hi[k], b[0], b[1]);
+          mma16816<T>(acc[j], lo[k], b[0], b[1]);
         }
       }
     }
 #pragma unroll
-    for (int m = 0; m < MW; ++m)
+    for (int h = 0; h < 2; ++h) {
+      if (row[h] < 0) continue;
+      T* dst = reinterpret_cast<T*>(p.out) + row[h] * p.out_stride;
 #pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        if (row[m][h] < 0) continue;
-        T* dst = reinterpret_cast<T*>(p.out) + row[m][h] * p.out_stride;
+      for (int c = 0; c < 2; ++c) {
+        const T* yt = reinterpret_cast<const T*>(yv[h][c]);
+        T o[8];
 #pragma unroll
-        for (int c = 0; c < 2; ++c) {
-          const T* yt = reinterpret_cast<const T*>(yv[m][h][c]);
-          T o[8];
+        for (int i = 0; i < 8; ++i) {
+          const float d = acc[4 * c + i / 2][2 * h + (i & 1)];
+          o[i] = tile.x >= 0 ? narrow<T>(fmaf(factor[h], d, widen<T>(yt[i]))) : yt[i];
+        }
+        if constexpr (VEC) {
+          if (n + 32 * c < p.N) *reinterpret_cast<uint4*>(dst + n + 32 * c) = *reinterpret_cast<const uint4*>(o);
+        } else {
 #pragma unroll
-          for (int i = 0; i < 8; ++i) {
-            const float d = acc[m][4 * c + i / 2][2 * h + (i & 1)];
-            o[i] = tile.x >= 0 ? narrow<T>(fmaf(factor[m][h], d, widen<T>(yt[i]))) : yt[i];
-          }
-          if constexpr (VEC) {
-            if (n + 32 * c < p.N) *reinterpret_cast<uint4*>(dst + n + 32 * c) = *reinterpret_cast<const uint4*>(o);
-          } else {
-#pragma unroll
-            for (int i = 0; i < 8; ++i)
-              if (n + 32 * c + i < p.N) dst[n + 32 * c + i] = o[i];
-          }
+          for (int i = 0; i < 8; ++i)
+            if (n + 32 * c + i < p.N) dst[n + 32 * c + i] = o[i];
         }
       }
+    }
   }
 }
 
@@ -735,8 +719,9 @@ int padded_rank(int64_t R) { return R <= 16 ? 16 : R <= 32 ? 32 : R <= 64 ? 64 :
 // elements (one 32-element step of each of four warps), at most 32 (the expand kernel
 // adds them up).  A function of the sizes alone, so the workspace can be sized first.
 constexpr int kSmsPlanned = 148;
+constexpr int part_rows(int tile) { return tile < 16 ? tile : 16; }
 int k_slices(int64_t M, int64_t K, int64_t S, int tile, int* k_slice) {
-  const int64_t tiles = ceil_div(M, tile) + (S < M ? S : M) / 2;
+  const int64_t tiles = ceil_div(M, part_rows(tile)) + (S < M ? S : M) / 2;
   int64_t slices = ceil_div(2 * kSmsPlanned, tiles);
   slices = slices > ceil_div(K, 128) ? ceil_div(K, 128) : slices;
   slices = slices > 32 ? 32 : slices < 1 ? 1 : slices;
@@ -765,60 +750,49 @@ int steps_of_one_per_sm(int64_t spans, const AdapterParams& p, int tile) {
   return steps;
 }
 
-template <typename T, int TILE, int RP, bool VEC>
-cudaError_t launch_adapter(AdapterParams p, const CUtensorMap* maps, cudaStream_t stream) {
-  if constexpr (TILE == 128 && VEC) {
+template <typename T, int RP, bool VEC>
+cudaError_t launch_adapter(AdapterParams p, const CUtensorMap* maps, int tile, cudaStream_t stream) {
+  const unsigned parts = tile == 128 ? 8 : 1;  // 16-row parts of a tile
+  if constexpr (VEC) {
     if (maps != nullptr) {
       using C = ExpandCfg<RP>;
-      cudaError_t e = ensure_smem_limit<adapter_shrink_kernel<T, 1, RP, VEC, true>>(shrink_shared(1, RP, true));
+      cudaError_t e = ensure_smem_limit<adapter_shrink_kernel<T, RP, VEC, true>>(shrink_shared(RP, true));
       if (e != cudaSuccess) return e;
-      e = launch_pdl(adapter_shrink_kernel<T, 1, RP, VEC, true>, dim3(p.tiles_cap, 8), 256,
-                                 shrink_shared(1, RP, true), stream, p);
+      e = launch_pdl(adapter_shrink_kernel<T, RP, VEC, true>, dim3(p.tiles_cap, 1, parts), 32 * shrink_warps(true),
+                     shrink_shared(RP, true), stream, p);
       if (e != cudaSuccess) return e;
       e = ensure_smem_limit<adapter_expand128_kernel<T, RP>>(C::SMEM);
       if (e != cudaSuccess) return e;
       const int64_t spans = ceil_div(p.N, 128);
-      p.col_steps = steps_of_one_per_sm(spans, p, TILE);
+      p.col_steps = steps_of_one_per_sm(spans, p, tile);
       return launch_pdl(adapter_expand128_kernel<T, RP>, dim3((unsigned)ceil_div(spans, p.col_steps), p.tiles_cap),
                         C::THREADS, C::SMEM, stream, maps[0], maps[1], maps[2], maps[3], p);
     }
   }
-  constexpr int WM = TILE == kFewRows ? 1 : TILE / 16;
-  cudaError_t e = launch_pdl(adapter_shrink_kernel<T, WM, RP, VEC, false>, dim3(p.tiles_cap, p.slices),
-                             32 * shrink_warps(WM, false), shrink_shared(WM, RP, false), stream, p);
+  cudaError_t e = launch_pdl(adapter_shrink_kernel<T, RP, VEC, false>, dim3(p.tiles_cap, p.slices, parts),
+                             32 * shrink_warps(false), shrink_shared(RP, false), stream, p);
   if (e != cudaSuccess) return e;
-  if constexpr (TILE == kFewRows && RP <= 64 && VEC) {
-    if (p.R % 8 == 0) {
-      const int64_t spans = ceil_div(p.N, 256);
-      p.col_steps = RP == 16 ? (steps_per_cta(2 * spans, p, TILE, 8) + 1) / 2 * 2 : steps_per_cta(spans, p, TILE, 8);
+  const int64_t spans = ceil_div(p.N, 256);
+  if constexpr (RP <= 64 && VEC) {
+    if (tile == kFewRows && p.R % 8 == 0) {
+      p.col_steps = RP == 16 ? (steps_per_cta(2 * spans, p, tile, 8) + 1) / 2 * 2 : steps_per_cta(spans, p, tile, 8);
       return launch_pdl(adapter_expand_few_kernel<T, RP>, dim3((unsigned)ceil_div(spans, p.col_steps), p.tiles_cap), 128, 0,
                         stream, p);
     }
   }
-  constexpr int MW = TILE == 128 ? 2 : 1;  // two 16-row blocks per warp halve the reads of `up`
-  constexpr int EWM = WM / MW;
-  const int64_t spans = ceil_div(p.N, 64 * (4 / EWM));
-  p.col_steps = steps_per_cta(spans, p, TILE, 8);
-  return launch_pdl(adapter_expand_kernel<T, EWM, MW, RP, VEC>, dim3((unsigned)ceil_div(spans, p.col_steps), p.tiles_cap),
+  p.col_steps = steps_per_cta(spans, p, part_rows(tile), 8);
+  return launch_pdl(adapter_expand_kernel<T, RP, VEC>, dim3((unsigned)ceil_div(spans, p.col_steps), p.tiles_cap, parts),
                     128, 0, stream, p);
 }
 
 template <typename T, bool VEC>
 cudaError_t dispatch(const AdapterParams& p, const CUtensorMap* maps, int tile, int rp, cudaStream_t s) {
-#define ACTUNE_ADAPTER(TILE)                                            \
-  switch (rp) {                                                         \
-    case 16: return launch_adapter<T, TILE, 16, VEC>(p, maps, s);         \
-    case 32: return launch_adapter<T, TILE, 32, VEC>(p, maps, s);         \
-    case 64: return launch_adapter<T, TILE, 64, VEC>(p, maps, s);         \
-    default: return launch_adapter<T, TILE, 128, VEC>(p, maps, s);        \
+  switch (rp) {
+    case 16: return launch_adapter<T, 16, VEC>(p, maps, tile, s);
+    case 32: return launch_adapter<T, 32, VEC>(p, maps, tile, s);
+    case 64: return launch_adapter<T, 64, VEC>(p, maps, tile, s);
+    default: return launch_adapter<T, 128, VEC>(p, maps, tile, s);
   }
-  if (tile == kFewRows) {
-    ACTUNE_ADAPTER(kFewRows)
-  } else if (tile == 16) {
-    ACTUNE_ADAPTER(16)
-  }
-  ACTUNE_ADAPTER(128)
-#undef ACTUNE_ADAPTER
 }
 
 // [n, rows, ranks] -> boxes of 64 ranks x 128 rows, 128-byte swizzled (ranks past the end
@@ -876,7 +850,9 @@ int actune_adapter_plan(const int32_t* slots, int64_t M, int64_t S, int tile, in
 size_t actune_adapter_workspace_size(int64_t M, int64_t K, int64_t S, int64_t R, int tile) {
   if (!valid_plan(M, S, tile) || M == 0 || K <= 0 || K > 0x7fffff00 || R <= 0 || R > kMaxRank) return 0;
   int k_slice = 0;
-  return 4 * ((size_t)k_slices(M, K, S, tile, &k_slice) * (size_t)M * (size_t)padded_rank(R) + (tile == 128 ? (size_t)M : 0));
+  const size_t rows = (size_t)M * (size_t)padded_rank(R), slices = (size_t)k_slices(M, K, S, tile, &k_slice);
+  // The tcgen05 form keeps one sum, as two 16-bit parts, and a factor per row.
+  return 4 * (tile == 128 && slices == 1 ? rows + (size_t)M : slices * rows);
 }
 
 int actune_adapter_add(const actune_adapter_args* a, void* stream) {
@@ -912,7 +888,11 @@ int actune_adapter_add(const actune_adapter_args* a, void* stream) {
   auto* cs = reinterpret_cast<cudaStream_t>(stream);
   CUtensorMap both[4] = {};
   const CUtensorMap* maps = nullptr;
-  if (vec && a->tile == 128 && a->R % 8 == 0) {  // rows of `up` a multiple of 16 bytes, as tensor maps want them
+  // Rows of `up` a multiple of 16 bytes, as tensor maps want them.  Low ranks with little to
+  // read and write are over sooner in 16-row parts, whose many small CTAs wait side by side:
+  // 800 rows 1024 -> 2560 at rank 16, 7.4 us and 10.9 us by tcgen05; 1024 rows 1024 -> 8192,
+  // 16.0 and 13.3 us; 1881 rows 312 -> 2560 at rank 64, 24.8 and 15.8 us.
+  if (vec && a->tile == 128 && a->R % 8 == 0 && (a->R > 32 || a->M * a->N >= 4 << 20)) {
     p.split = a->workspace;
     p.factor = reinterpret_cast<float*>(a->workspace) + a->M * rp;
     int st = encode_ranks(&both[0], a->dtype, a->up, a->R, a->N, a->S);
