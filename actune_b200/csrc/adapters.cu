@@ -18,7 +18,7 @@
 // latency: `up` asked for before v is there), 16 rows by mma.sync, and 128 rows on
 // tcgen05 with y and out as boxes by TMA (their time is that traffic; with little of it
 // tiles of 128 take the 16-row form in parts).  16 requests of 304
-// tokens, 2048 -> 32768, rank 64: @VLM@, the floor of its bytes 114 us.
+// tokens, 2048 -> 32768, rank 64: 178 us, the floor of its bytes 114 us.
 #include "serving.cuh"
 
 namespace actune {
