@@ -105,7 +105,7 @@ struct AdapterParams {
   const float* scale;
   const int32_t* plan;
   void* out;
-  float* v;       // [slices, M, RP] partial sums of down x, rows in plan order; or, for tiles of 128,
+  float* v;       // [slices, M, RP] partial sums of down x, rows in plan order; or, for the tcgen05 form,
   void* split;    // [2, M, RP]: down x as hi and lo parts, and
   float* factor;  // [M]: what a row's product with `up` is multiplied by
   int boxes;      // y and out have tensor maps
@@ -729,7 +729,7 @@ int k_slices(int64_t M, int64_t K, int64_t S, int tile, int* k_slice) {
   return (int)ceil_div(K, *k_slice);
 }
 
-// 64- or 128-column steps a CTA walks: 8 CTAs per SM and more before they get longer.
+// 256-column steps a CTA walks: 8 CTAs per SM and more before they get longer.
 int steps_per_cta(int64_t spans, const AdapterParams& p, int tile, int most) {
   const int64_t tiles = ceil_div(p.M, tile) + (p.S < p.M ? p.S : p.M) / 2;
   const int64_t steps = spans * tiles / (kSmsPlanned * 8);
