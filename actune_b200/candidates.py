@@ -146,7 +146,7 @@ class CandidatePolicy(torch.nn.Module):
     def sample(self, noise, state, prefix_cache, graph=False):
         """Action candidates [envs, candidates, horizon, action_dim] from noise of that
         shape.  ``graph``: replay a captured step (adapters may be routed anew between
-        calls; the captured graph reads the same plan)."""
+        calls: the plan is an input of the graph)."""
         dt = torch.full((), -1.0 / self.steps, dtype=torch.float32, device=noise.device)
         time = torch.full((), 1.0, dtype=torch.float32, device=noise.device)
         self.step_graph.enabled = graph

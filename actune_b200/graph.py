@@ -7,7 +7,8 @@ contract:
 
 * a call is identified by the argument pytree, every tensor leaf's shape, stride,
   dtype and device (non-tensor leaves by type and repr), and the active mode of
-  every bank layer under the current precision profile;
+  every bank layer under the current precision profile; under an ``adapter_scope``
+  also by the sizes of its plan (rows, adapters, tile);
 * a new identity is warmed up twice on a side stream and then captured, until
   ``max_graphs`` graphs exist; beyond that the call runs eagerly and counts a
   fallback (no eviction);
@@ -24,7 +25,9 @@ How it is organised here: calls are grouped by input signature into *slots*.  A
 slot owns one set of static input buffers, shared by every precision
 configuration captured for that signature, so switching q00/q01/q11/q10 between
 calls copies the inputs into the same buffers and replays another graph -- no
-per-configuration input copies.  Literal constants are intercepted with a
+per-configuration input copies.  The active adapter plan is an input like the
+others: a slot has a plan of its own, which the captures read and which takes the
+active one's contents before every replay.  Literal constants are intercepted with a
 ``TorchFunctionMode`` while warming up and capturing.  With ``shared_a8`` the
 sibling projections of a captured function share one activation quantization
 (the shared activation scope of kernels.grouped and the tokenwise A8/A4 cache).
@@ -32,13 +35,14 @@ sibling projections of a captured function share one activation quantization
 from __future__ import annotations
 
 from contextlib import ExitStack, contextmanager
-from dataclasses import dataclass, field
+from dataclasses import dataclass, field, replace
 from typing import Any
 
 import torch
 from torch.overrides import TorchFunctionMode
 from torch.utils import _pytree as pytree
 
+from .adapters import active_adapter_plan, adapter_scope
 from .kernels._tokenwise import shared_a8_cache_scope
 from .kernels.grouped import shared_activation_scope
 from .precision import active_precision_profile
@@ -88,6 +92,7 @@ class _Capture:
 @dataclass
 class _Slot:
     statics: list         # static leaves (tensors cloned once) shared by the slot's captures
+    plan: Any = None      # the adapter plan the captures read; None: no adapters
     captures: dict = field(default_factory=dict)   # per-layer modes -> _Capture
 
 
@@ -106,7 +111,8 @@ class GraphReplay:
     # ------------------------------------------------------------------ identity
     @staticmethod
     def _signature(leaves, tree):
-        sig = []
+        plan = active_adapter_plan()
+        sig = [] if plan is None else [("adapter plan", plan.rows, plan.adapters, plan.tile, str(plan.buffer.device))]
         for x in leaves:
             if isinstance(x, torch.Tensor):
                 sig.append((tuple(x.shape), tuple(x.stride()), str(x.dtype), str(x.device)))
@@ -119,7 +125,8 @@ class GraphReplay:
         return tuple(m.assignments[profile or m.default_profile] for m in self.layers.values())
 
     def key(self, leaves, tree):
-        """The identity of a call: (pytree, leaf signature, every layer's active mode)."""
+        """The identity of a call: (pytree, signature of the leaves and of the active adapter
+        plan, every layer's active mode)."""
         tree_s, sig = self._signature(leaves, tree)
         return tree_s, sig, self._modes()
 
@@ -149,6 +156,7 @@ class GraphReplay:
         leaves, tree = pytree.tree_flatten((args, kwargs))
         slot_key = self._signature(leaves, tree)
         modes = self._modes()
+        plan = active_adapter_plan()
         slot = self._slots.get(slot_key)
         capture = None if slot is None else slot.captures.get(modes)
         if capture is None:
@@ -156,12 +164,16 @@ class GraphReplay:
                 self.fallbacks += 1
                 return self.function(*args, **kwargs)
             if slot is None:
-                slot = _Slot([x.clone() if isinstance(x, torch.Tensor) else x for x in leaves])
+                slot = _Slot([x.clone() if isinstance(x, torch.Tensor) else x for x in leaves],
+                             None if plan is None else replace(plan, buffer=plan.buffer.clone()))
                 self._slots[slot_key] = slot
-            capture = slot.captures[modes] = self._record(slot, tree)
+            with adapter_scope(slot.plan):
+                capture = slot.captures[modes] = self._record(slot, tree)
         for src, dst in zip(leaves, slot.statics, strict=True):
             if isinstance(src, torch.Tensor) and src.data_ptr() != dst.data_ptr():
                 dst.copy_(src)
+        if plan is not None:
+            slot.plan.buffer.copy_(plan.buffer)
         capture.graph.replay()
         for name, (calls, elements) in capture.deltas.items():
             layer = self.layers[name]

@@ -71,7 +71,8 @@ def gated_norm(x, residual, pre_weight, *, post_weight=None, gate=None, shift=No
 class AdapterPlan:
     """The rows of a batch sorted by adapter slot (made by ``adapter_plan``; read by
     every ``adapter_add`` the batch passes through).  ``update`` routes the same number
-    of rows anew into the same buffer, so a captured graph follows it."""
+    of rows anew into the same buffer, so a captured graph that reads it follows; the plan
+    has to live as long as such a graph."""
 
     buffer: torch.Tensor
     rows: int

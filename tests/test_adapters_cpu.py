@@ -1,8 +1,12 @@
 """Adapter slots and scopes on the CPU: installing, loading, refusals, pass-through."""
+import types
+
 import pytest
 import torch
 
+from actune_b200 import ops
 from actune_b200.adapters import AdaptedLinear, active_adapter_plan, adapter_scope, install_adapters
+from actune_b200.graph import GraphReplay, _Capture
 
 
 def model():
@@ -80,3 +84,65 @@ def test_a_bank_projection_keeps_its_format():
 
     a = AdaptedLinear(Resident(12, 20), slots=1, rank=8)
     assert a.padding == 4 and hasattr(a, "active_backend") and a.active_backend() == "backend"
+
+
+def plan_of(slots, adapters=4, tile=16):
+    """A plan as far as a host test needs one: its buffer holds the slots."""
+    return ops.AdapterPlan(torch.tensor(slots, dtype=torch.int32), len(slots), adapters, tile)
+
+
+class HostReplay(GraphReplay):
+    """Captures as a CUDA graph does, on the host: what was active while recording is
+    what every replay reads, by the buffer it had then."""
+
+    def _record(self, slot, tree):
+        plan = active_adapter_plan()
+        output = []
+        graph = types.SimpleNamespace(
+            plan=plan, replay=lambda: output.__setitem__(slice(None), [None if plan is None else plan.buffer.tolist()]))
+        return _Capture(graph, output, {})
+
+
+def test_graph_key_holds_the_sizes_of_the_active_plan():
+    replay = GraphReplay(lambda x: x, {})
+    leaves, tree = torch.utils._pytree.tree_flatten(((torch.zeros(2, 3),), {}))
+    keys = [replay.key(leaves, tree)]
+    for plan in (plan_of([0, 1]), plan_of([0, 1, 2]), plan_of([0, 1], adapters=5), plan_of([0, 1], tile=4)):
+        with adapter_scope(plan):
+            keys.append(replay.key(leaves, tree))
+            with adapter_scope(None):
+                assert replay.key(leaves, tree) == keys[0]
+    assert len(set(keys)) == 5
+    with adapter_scope(plan_of([1, 0])):  # another routing of the same sizes replays the same graph
+        assert replay.key(leaves, tree) == keys[1]
+
+
+@pytest.mark.parametrize("first", ["scope", "none"])
+def test_a_replay_runs_the_active_plan_and_none_outside_a_scope(first):
+    replay = HostReplay(lambda x: x, {})
+    replay.enabled = True
+    x = torch.zeros(2, 3)
+    a, b = plan_of([0, 1]), plan_of([3, -1])
+    if first == "none":
+        assert replay(x) == [None]
+    for plan in (a, b, a):
+        with adapter_scope(plan):
+            assert replay(x) == [plan.buffer.tolist()]
+            with adapter_scope(None):
+                assert replay(x) == [None]
+        assert replay(x) == [None]
+    a.buffer.copy_(torch.tensor([2, 2]))  # as AdapterPlan.update does
+    with adapter_scope(a):
+        assert replay(x) == [[2, 2]]
+    assert len(replay.graphs) == 2 and replay.fallbacks == 0
+
+
+def test_a_capture_reads_a_plan_of_its_own():
+    """Whatever becomes of the plan it was captured under."""
+    replay = HostReplay(lambda x: x, {})
+    replay.enabled = True
+    plan = plan_of([0, 1])
+    with adapter_scope(plan):
+        replay(torch.zeros(2, 3))
+    (capture,) = replay.graphs.values()
+    assert capture.graph.plan.buffer.data_ptr() != plan.buffer.data_ptr()

@@ -164,3 +164,45 @@ def test_empty_batch_and_update_in_a_graph():
         slots.copy_(random_slots(48, 5, seed))
         graph.replay()
         check(out, y, x, down, up, scale, slots)
+
+
+def test_graph_replay_follows_the_scope():
+    """Captured under a plan or under none, then called under others and with the first gone."""
+    from actune_b200 import ops
+    from actune_b200.adapters import AdaptedLinear, adapter_scope
+    from actune_b200.graph import GraphReplay
+    linear = torch.nn.Linear(64, 96, bias=False, device="cuda", dtype=torch.bfloat16)
+    layer = AdaptedLinear(linear, slots=3, rank=8)
+    g = torch.Generator(device="cuda").manual_seed(1)
+    for slot in range(3):
+        layer.load(slot, torch.randn(8, 64, device="cuda", generator=g), torch.randn(96, 8, device="cuda", generator=g))
+    x = torch.randn(40, 64, device="cuda", generator=g).bfloat16()
+    with torch.inference_mode():
+        y = linear(x)
+        for captured in (0, None):
+            replay = GraphReplay(layer, {})
+            replay.enabled = True
+            slots = [random_slots(40, 3, seed) for seed in range(3)]
+            plans = [ops.adapter_plan(s, 3) for s in slots]
+
+            def call(of):
+                with adapter_scope(None if of is None else plans[of]):
+                    out = replay(x)
+                if of is None:
+                    assert torch.equal(out, y)
+                else:
+                    check(out, y, x, layer.down, layer.up, layer.scale, slots[of])
+
+            for of in (captured, 1, None, 0, 2, None):
+                call(of)
+            assert torch.equal(replay(x), y)  # outside any scope
+            # The first plan goes, and its memory is something else's.
+            plans[0] = slots[0] = None
+            others = [torch.full_like(plans[1].buffer, -1) for _ in range(64)]
+            for of in (1, None, 2):
+                call(of)
+            plans[2].update(slots[1])
+            slots[2] = slots[1]
+            call(2)
+            assert len(replay.graphs) == 2 and replay.fallbacks == 0 and len(others) == 64
+            replay.release()
