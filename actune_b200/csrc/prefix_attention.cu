@@ -33,8 +33,9 @@
 //                   O += P V (P in tensor memory, V as the MN-major operand)
 // S of the next block is computed while this block's softmax runs (two score buffers a
 // row tile).  O is rescaled only when the maximum has grown by more than 2^8 since the
-// last time: until then p stays below 2^8, which the 16-bit types and the fp32 sums hold,
-// and l and O carry the same factor.
+// last time: until then p stays below 2^8, and l and O carry the same factor.  fp16 has 5
+// exponent bits: its p, l and O carry a further 2^7 (p below 2^15), so that a long tail of
+// keys far below the maximum is weighed down to 2^-32 of it, not to 2^-25.
 //
 // Bounds: at head sizes up to 128 a block of 64 keys asks 128 rows x 64 exponentials of
 // each tile, as long as its products; with the softmax's latency between the two products
@@ -50,6 +51,8 @@ namespace {
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kRescale = 8.f;  // growth of the maximum (log2) that O is rescaled for
 constexpr int kSiteAttn = 300;
+template <typename T>
+constexpr float kRoom = std::is_same<T, __half>::value ? 7.f : 0.f;  // log2 of what p, l and O carry
 
 // Tiles by sequence; stacked tiles for the prefix and tiles by sequence for the own keys;
 // stacked tiles for both.
@@ -684,7 +687,7 @@ __global__ void __launch_bounds__(AttnCfg<DP, NT>::WARPS * 32, 1)
         // found beside them.  Only where that is more than 2^8 above (or there is none yet)
         // O and l are brought to the new maximum and the exponentials taken again.
         for (bool again = false;; again = true) {
-          const float ref = m == -INFINITY ? 0.f : m;
+          const float ref = m == -INFINITY ? 0.f : m - kRoom<T>;
           const float2 c2 = make_float2(p.scale, p.scale), r2 = make_float2(-ref, -ref);
           float top[2] = {-INFINITY, -INFINITY};
           float2 add[2] = {};

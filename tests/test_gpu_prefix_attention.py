@@ -253,3 +253,49 @@ def test_empty_batch():
     q, pk, pv, k, v = operands(2, 3, 4, 2, 64, 1, 10, 4, torch.bfloat16, 1)
     assert ops.shared_prefix_attention(q[:0], pk, pv, k[:0], v[:0]).shape == (0, 3, 4, 64)
     assert ops.shared_prefix_attention(q[:, :0], pk, pv, k, v).shape == (2, 0, 4, 64)
+
+
+@pytest.mark.parametrize("below", [16.0, 21.5, 23.4, 25.1, 27.0])
+@pytest.mark.parametrize("B,T,H,KV,G,P,S,D", [
+    (1, 1, 4, 4, 1, 32768, 0, 64),     # by sequence, parts joined
+    (24, 1, 8, 2, 1, 32768, 5, 128),   # stacked
+    (120, 5, 8, 1, 3, 8192, 64, 256),  # mixed tiles
+    (2, 200, 4, 4, 2, 8192, 64, 64),
+])
+def test_a_long_tail_of_keys_far_below_a_sink_in_fp16(B, T, H, KV, G, P, S, D, below):
+    """One key with value 0 ahead of all others by `below` (log2): the output is what the
+    tail weighs, and none of it may fall under fp16's range on the way.
+
+    The tail's probabilities all are about 2^-below of the sink's.  Each is rounded to fp16
+    relative to a maximum of 2^7, in steps of 2^-24 at least: by 2^-32 of the sink's at
+    most, beside the relative error of `check`'s bound."""
+    g = torch.Generator(device="cuda").manual_seed(int(10 * below))
+
+    def near(*shape, mean):  # exact in fp16 and of 5 values only: products and sums of scores are exact
+        return (torch.randint(-2, 3, shape, device="cuda", generator=g) * 2.0 ** -5 + mean).half()
+
+    q = torch.zeros(B, T, H, D, device="cuda").half()
+    q[..., 0] = 1.0
+    pk, k = torch.zeros(G, P, KV, D, device="cuda").half(), torch.zeros(B, S, KV, D, device="cuda").half()
+    pk[..., 0], k[..., 0] = near(G, P, KV, mean=-below), near(B, S, KV, mean=-below)
+    pk[:, 0] = 0.0  # the sink
+    pv, v = near(G, P, KV, D, mean=1.0), near(B, S, KV, D, mean=1.0)
+    pv[:, 0] = 0.0
+    scale = 0.6931471805599453  # scores in log2
+    from actune_b200 import _lib, ops
+    out = ops.shared_prefix_attention(q, pk, pv, k, v, scale=scale)
+    assert _lib.device_error() == (0, 0)
+    for b in range(B):
+        keys, values = torch.cat([pk[b * G // B], k[b]]).double(), torch.cat([pv[b * G // B], v[b]]).double()
+        w = torch.exp2(keys[..., 0]).t()                       # KV, n
+        p = w / w.sum(1, keepdim=True)
+        ref = torch.einsum("kn,nkd->kd", p, values)
+        mass = torch.einsum("kn,nkd->kd", p, values.abs())
+        n = keys.shape[0]
+        e = (D / 16 + 4) * 2.0 ** -23 * below + 2.0 ** -21 * (1 + below)
+        tol = (UNIT[torch.float16] + 2 * e + (n / 16 + 64) * 2.0 ** -23) * mass \
+            + 2.0 ** -32 / w.sum(1)[:, None] * torch.einsum("nkd->kd", values.abs())
+        got = out[b].double().view(T, KV, H // KV, D)
+        bad = (got - ref[None, :, None]).abs() > (UNIT[torch.float16] * ref.abs() + tol * (1 + UNIT[torch.float16])
+                                                  + TINY[torch.float16])[None, :, None]
+        assert not bad.any(), f"sequence {b}: {float((got - ref[None, :, None]).abs().max())} of {float(ref.abs().max())}"
