@@ -51,7 +51,8 @@ class AdaptedLinear(torch.nn.Module):
 
     ``projection`` is any module from [..., in_features] to [..., out_features] (a bank's
     ResidentLinear, an nn.Linear) whose output nobody else holds: the adapters are added
-    to it in place."""
+    to it in place.  They have no backward: in a scope, an output that requires a gradient
+    is refused (RuntimeError), so such a projection is run under ``torch.no_grad()``."""
 
     def __init__(self, projection, slots, rank, dtype=torch.bfloat16, device=None):
         super().__init__()

@@ -8,6 +8,7 @@
 // status of the C entry.  Operands that do not fit raise RuntimeError; no C++ exception
 // leaves the module.
 #include <ATen/ATen.h>
+#include <c10/core/GradMode.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
 #include <torch/csrc/autograd/python_variable.h>
@@ -81,6 +82,16 @@ Tensor empty(at::IntArrayRef size, at::ScalarType dtype, c10::Device device) {
 }
 int64_t row_stride(const Tensor& t) { return t.size(0) > 1 ? t.stride(0) : t.size(1); }
 void* stream(c10::Device device) { return c10::cuda::getCurrentCUDAStream(device.index()).stream(); }
+
+// `out` given by the caller is written behind autograd's back.  Refused where a gradient
+// would be taken through it; otherwise its version tells a backward pass that saved it.
+void check_written(const Tensor& out) {
+  REQUIRE(!(c10::GradMode::is_enabled() && out.requires_grad()),
+          "out requires a gradient, and the serving operators have no backward: run them under torch.no_grad()");
+}
+void mark_written(const Tensor& out) {
+  if (!out.is_inference()) out.unsafeGetTensorImpl()->bump_version();
+}
 
 PyObject* outputs(std::initializer_list<Tensor> list) {
   PyObject* tuple = PyTuple_New((Py_ssize_t)list.size());
@@ -193,6 +204,7 @@ PyObject* adapter_add(PyObject* const* a) {
     // Rows of `out` that overlap would be written while others read them.
     REQUIRE(rows <= 1 || out.stride(0) >= n, "the rows of out must not overlap");
     REQUIRE(n <= 1 || out.stride(1) == 1, "the last dimension must be contiguous");
+    check_written(out);
   }
   REQUIRE((k <= 1 || x.stride(1) == 1) && (n <= 1 || y.stride(1) == 1), "the last dimension must be contiguous");
   const c10::Device device =
@@ -213,6 +225,7 @@ PyObject* adapter_add(PyObject* const* a) {
   g.x_stride = row_stride(x), g.y_stride = row_stride(y), g.out_stride = row_stride(out);
   g.tile = (int32_t)tile, g.dtype = dtype_code(dtype);
   const int status = actune_adapter_add(&g, stream(device));
+  mark_written(out);
   return status != ACTUNE_OK ? PyLong_FromLong(status) : THPVariable_Wrap(out);
 }
 
@@ -256,6 +269,7 @@ PyObject* shared_prefix_attention(PyObject* const* a) {
   REQUIRE(g.D == 1 || (q.stride(3) == 1 && pk.stride(3) == 1 && pv.stride(3) == 1 && k.stride(3) == 1 &&
                        v.stride(3) == 1),
           "the last dimension must be contiguous");
+  if (out.defined()) check_written(out);
   const c10::Device device =
       one_device(q, {{"prefix_k", &pk}, {"prefix_v", &pv}, {"k", &k}, {"v", &v}, {"starts", &starts},
                      {"prefix_lens", &plens}, {"lens", &lens}, {"out", &out}});
@@ -284,6 +298,7 @@ PyObject* shared_prefix_attention(PyObject* const* a) {
   g.v_b = v.stride(0), g.v_s = v.stride(1), g.v_h = v.stride(2);
   g.scale = (float)scale, g.dtype = dtype_code(dtype), g.causal = truth(a[8]);
   const int status = actune_prefix_attention(&g, stream(device));
+  mark_written(out);
   return status != ACTUNE_OK ? PyLong_FromLong(status) : THPVariable_Wrap(out);
 }
 

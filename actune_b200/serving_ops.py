@@ -9,7 +9,9 @@ re-exported by ``actune_b200.ops``.
 
 Conventions of ``ops``: tensors on one CUDA device, that device's current stream,
 RuntimeError for operands that do not fit, outputs and scratch from torch's allocator
-(so they belong to the stream the call runs on).  Nothing here synchronises.  The checks
+(so they belong to the stream the call runs on).  Nothing here synchronises, and nothing
+has a backward: outputs carry no gradient, and an ``out`` that requires one is refused
+(RuntimeError) while gradients are enabled.  The checks
 and the C-ABI call are in the compiled module ``_serving`` (csrc/torch/serving.cpp).
 """
 from __future__ import annotations

@@ -146,3 +146,22 @@ def test_a_capture_reads_a_plan_of_its_own():
         replay(torch.zeros(2, 3))
     (capture,) = replay.graphs.values()
     assert capture.graph.plan.buffer.data_ptr() != plan.buffer.data_ptr()
+
+
+def test_adapters_are_refused_where_a_gradient_would_pass_them_by():
+    """They are added behind autograd's back, whose gradient would lack their term."""
+    layer = AdaptedLinear(torch.nn.Linear(12, 20, dtype=torch.bfloat16), slots=4, rank=8)
+    x = torch.zeros(2, 12).bfloat16()
+    with adapter_scope(ops.AdapterPlan(torch.zeros(64, dtype=torch.int32), 2, 4, 16)):
+        with pytest.raises(RuntimeError, match="no backward"):
+            layer(x)  # the projection's weight requires a gradient
+        for context in (torch.no_grad, torch.inference_mode):
+            with context(), pytest.raises(RuntimeError, match="CUDA required"):
+                layer(x)
+        with adapter_scope(None):
+            assert layer(x).requires_grad
+        layer.requires_grad_(False)
+        with pytest.raises(RuntimeError, match="no backward"):
+            layer(x.clone().requires_grad_())
+        with pytest.raises(RuntimeError, match="CUDA required"):
+            layer(x)

@@ -206,3 +206,23 @@ def test_graph_replay_follows_the_scope():
             call(2)
             assert len(replay.graphs) == 2 and replay.fallbacks == 0 and len(others) == 64
             replay.release()
+
+
+def test_autograd_sees_what_out_overwrites():
+    """A value saved for a backward pass and then written to is refused by that pass."""
+    from actune_b200 import ops
+    y, x, down, up, scale = operands(20, 64, 64, 2, 8, torch.bfloat16, 3)
+    w = torch.ones(64, device="cuda", dtype=torch.bfloat16, requires_grad=True)
+    plan = ops.adapter_plan(random_slots(20, 2, 1), 2)
+    for out in (None, y):
+        loss = (w * y).sum()
+        ops.adapter_add(y, x, down, up, scale, plan, out=out)
+        if out is None:
+            loss.backward()
+        else:
+            with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+                loss.backward()
+    with torch.inference_mode():
+        z = y * 1.0
+        ops.adapter_add(z, x, down, up, scale, plan, out=z)
+    ops.adapter_add(z, x, down, up, scale, plan, out=z)  # outside too: an inference tensor has no version

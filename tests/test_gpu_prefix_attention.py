@@ -299,3 +299,22 @@ def test_a_long_tail_of_keys_far_below_a_sink_in_fp16(B, T, H, KV, G, P, S, D, b
         bad = (got - ref[None, :, None]).abs() > (UNIT[torch.float16] * ref.abs() + tol * (1 + UNIT[torch.float16])
                                                   + TINY[torch.float16])[None, :, None]
         assert not bad.any(), f"sequence {b}: {float((got - ref[None, :, None]).abs().max())} of {float(ref.abs().max())}"
+
+
+@pytest.mark.parametrize("B,T,D", [(4, 50, 128), (24, 1, 64), (100, 9, 256), (3, 2, 20)])
+def test_out_is_written_and_returned(B, T, D):
+    from actune_b200 import ops
+    args = operands(B, T, 8, 2, D, 1, 700, 30, torch.bfloat16, 31)
+    want = ops.shared_prefix_attention(*args)
+    room = torch.full((B + 2, T, 8, D), 7.0, device="cuda", dtype=torch.bfloat16)
+    out = room[1:-1]
+    assert ops.shared_prefix_attention(*args, out=out) is out and torch.equal(out, want)
+    assert (room[0] == 7).all() and (room[-1] == 7).all()
+    w = torch.ones(D, device="cuda", dtype=torch.bfloat16, requires_grad=True)
+    loss = (w * out).sum()
+    ops.shared_prefix_attention(*args, out=out)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        loss.backward()
+    for wrong in (room, out.transpose(2, 3).contiguous().transpose(2, 3), out.half()):
+        with pytest.raises(RuntimeError, match="out must be contiguous and match q"):
+            ops.shared_prefix_attention(*args, out=wrong)

@@ -142,3 +142,18 @@ def test_adapter_add_refuses_operands_that_do_not_fit():
         ops.adapter_plan(torch.zeros(4, dtype=torch.int64), 2)
     with pytest.raises(RuntimeError, match="CUDA required"):
         ops.adapter_plan(torch.zeros(4, dtype=torch.int32), 2)
+
+
+def test_outputs_that_require_a_gradient_are_refused():
+    y, x, s = torch.zeros(6, 32).half(), torch.zeros(6, 16).half(), torch.ones(2)
+    down, up = torch.zeros(2, 4, 16).half(), torch.zeros(2, 32, 4).half()
+    plan = ops.AdapterPlan(torch.zeros(64, dtype=torch.int32), 6, 2, 16)
+    q, pk, k = torch.zeros(4, 2, 4, 64).half(), torch.zeros(2, 9, 2, 64).half(), torch.zeros(4, 5, 2, 64).half()
+    for call in (lambda out: ops.adapter_add(y, x, down, up, s, plan, out=out(y)),
+                 lambda out: ops.shared_prefix_attention(q, pk, pk, k, k, out=out(q))):
+        with pytest.raises(RuntimeError, match="no backward"):
+            call(lambda t: t.clone().requires_grad_())
+        with pytest.raises(RuntimeError, match="no backward"):
+            call(lambda t: t.clone().requires_grad_() * 2)
+        with torch.no_grad(), pytest.raises(RuntimeError, match="CUDA required"):
+            call(lambda t: t.clone().requires_grad_())
