@@ -702,6 +702,8 @@ __global__ void __launch_bounds__(ExpandCfg<RP>::THREADS, 1)
           *reinterpret_cast<uint4*>(reinterpret_cast<T*>(p.out) + to * p.out_stride + col + 8 * piece) =
               *reinterpret_cast<const uint4*>(stage + (piece >> 3) * (128 * 128) + (32 * quarter + rr) * 128 + (((piece & 7) ^ (rr & 7)) << 4));
         }
+        // The slot's next rows may come as a box: behind what was read and written here.
+        fence_proxy_async_smem();
         __syncwarp();
         if (lane == 0) mbar_arrive(&y_empty[slot]);
       }

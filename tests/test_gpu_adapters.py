@@ -226,3 +226,89 @@ def test_autograd_sees_what_out_overwrites():
         z = y * 1.0
         ops.adapter_add(z, x, down, up, scale, plan, out=z)
     ops.adapter_add(z, x, down, up, scale, plan, out=z)  # outside too: an inference tensor has no version
+
+
+# The form of long prompts: tiles of 128 rows, y and out as boxes of 32 consecutive rows.
+# Requests of every remainder of a box and of a tile, some without an adapter, over enough
+# columns (the last step's 8 of 128) for a block to go through its rings several times.
+RUNS = (304, 81, 50, 128, 16, 33, 700, 1, 31, 352, 15, 97, 304, 112)
+
+
+def run_slots(rows, slots, seed):
+    g = torch.Generator().manual_seed(seed)
+    out = []
+    while len(out) < rows:
+        for n in RUNS:
+            out += [int(torch.randint(-1, slots, (1,), generator=g))] * n
+    return torch.tensor(out[:rows], dtype=torch.int32).cuda()
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("rank", [8, 16, 24, 32, 40, 64, 104, 128])
+@pytest.mark.parametrize("in_place", [False, True])
+def test_long_prompts(in_place, rank, dtype):
+    from actune_b200 import _lib, ops
+    rows, n = 4864, 8200
+    y, x, down, up, scale = operands(rows, 136, n, 16, rank, dtype, rank)
+    index = run_slots(rows, 16, rank)
+    plan = ops.adapter_plan(index, 16)
+    assert plan.tile == 128
+    out = y.clone() if in_place else None
+    got = ops.adapter_add(y if out is None else out, x, down, up, scale, plan, out=out)
+    assert _lib.device_error() == (0, 0)
+    check(got, y, x, down, up, scale, index)
+
+
+@pytest.mark.parametrize("rank", [16, 64, 128])
+@pytest.mark.parametrize("columns", [72, 1024, 2056])
+def test_long_prompts_strided_and_in_place(columns, rank):
+    from actune_b200 import ops
+    rows = 4200
+    y, x, down, up, scale = operands(rows, 264, columns, 7, rank, torch.bfloat16, columns)
+    index = run_slots(rows, 7, 5)
+    plan = ops.adapter_plan(index, 7)
+    wide = torch.randn(rows, columns + 64, device="cuda").bfloat16()
+    view = wide[:, 8:columns + 8]
+    view.copy_(y)
+    around = wide.clone()
+    ops.adapter_add(view, torch.cat([x, x], 1)[:, 264:], down, up, scale, plan, out=view)
+    check(view, y, x, down, up, scale, index)
+    around[:, 8:columns + 8] = view
+    assert torch.equal(around, wide)
+    one = y[:1].expand(rows, -1)  # one row of y for all
+    check(ops.adapter_add(one, x, down, up, scale, plan), one, x, down, up, scale, index)
+
+
+@pytest.mark.parametrize("in_place", [False, True])
+@pytest.mark.parametrize("rank", [16, 64])
+def test_long_prompts_keep_non_finite_rows_alone(rank, in_place):
+    from actune_b200 import ops
+    rows = 4864
+    y, x, down, up, scale = operands(rows, 128, 2048, 16, rank, torch.bfloat16, 9)
+    index = run_slots(rows, 16, 4)
+    plan = ops.adapter_plan(index, 16)
+    clean = ops.adapter_add(y, x, down, up, scale, plan)
+    x[5], y[700, 9], x[2000, 3], down[3] = float("nan"), float("inf"), float("inf"), float("nan")
+    index[[5, 2000]] = 1
+    index[700] = -1
+    plan.update(index)
+    out = y.clone()
+    out = ops.adapter_add(out if in_place else y, x, down, up, scale, plan, out=out if in_place else None)
+    assert out[5].isnan().all() and torch.equal(out[700], y[700]) and not out[2000].isfinite().any()
+    assert out[index == 3].isnan().all()
+    keep = (index != 3)
+    keep[[5, 700, 2000]] = False
+    assert torch.equal(out[keep], clean[keep])
+
+
+def test_long_prompts_of_large_and_small_magnitudes_in_fp16():
+    from actune_b200 import ops
+    for factor in (2.0 ** 9, 2.0 ** -12):
+        for rank, n in ((16, 21000), (64, 328)):
+            y, x, down, up, scale = operands(200, 512, n, 2, rank, torch.float16, 6)
+            x, up = (x * factor).half(), (up / (factor * 16)).half()
+            down = (down * 64).half() if factor > 1 else down
+            index = run_slots(200, 2, 6)
+            plan = ops.adapter_plan(index, 2)
+            assert plan.tile == 128
+            check(ops.adapter_add(y, x, down, up, scale, plan), y, x, down, up, scale, index)
