@@ -26,6 +26,7 @@ namespace {
 
 constexpr int kMaxSlots = 8191;
 constexpr int kMaxRank = 128;
+constexpr int64_t kMostColumns = 0x7fff0000;  // of N and K: the indexes of a block's steps behind them are 32-bit
 constexpr int kFewRows = 4;
 constexpr int kHeader = 4;  // plan: tile count, then three padding words
 
@@ -850,7 +851,7 @@ int actune_adapter_plan(const int32_t* slots, int64_t M, int64_t S, int tile, in
 }
 
 size_t actune_adapter_workspace_size(int64_t M, int64_t K, int64_t S, int64_t R, int tile) {
-  if (!valid_plan(M, S, tile) || M == 0 || K <= 0 || K > 0x7fffff00 || R <= 0 || R > kMaxRank) return 0;
+  if (!valid_plan(M, S, tile) || M == 0 || K <= 0 || K > kMostColumns || R <= 0 || R > kMaxRank) return 0;
   int k_slice = 0;
   const size_t rows = (size_t)M * (size_t)padded_rank(R), slices = (size_t)k_slices(M, K, S, tile, &k_slice);
   // The tcgen05 form keeps one sum, as two 16-bit parts, and a factor per row.
@@ -859,7 +860,7 @@ size_t actune_adapter_workspace_size(int64_t M, int64_t K, int64_t S, int64_t R,
 
 int actune_adapter_add(const actune_adapter_args* a, void* stream) {
   if (a == nullptr || a->struct_bytes != sizeof(actune_adapter_args)) return ACTUNE_ERR_INVALID_VALUE;
-  if (!valid_plan(a->M, a->S, a->tile) || a->N < 0 || a->N > 0x7fffff00 || a->K <= 0 || a->K > 0x7fffff00 ||
+  if (!valid_plan(a->M, a->S, a->tile) || a->N < 0 || a->N > kMostColumns || a->K <= 0 || a->K > kMostColumns ||
       a->R <= 0 || a->R > kMaxRank || a->x_stride < 0 || a->y_stride < 0 || a->out_stride < a->N ||
       (a->dtype != ACTUNE_DTYPE_F16 && a->dtype != ACTUNE_DTYPE_BF16))
     return ACTUNE_ERR_INVALID_VALUE;

@@ -157,3 +157,16 @@ def test_outputs_that_require_a_gradient_are_refused():
             call(lambda t: t.clone().requires_grad_() * 2)
         with torch.no_grad(), pytest.raises(RuntimeError, match="CUDA required"):
             call(lambda t: t.clone().requires_grad_())
+
+
+def test_adapter_sizes_whose_last_step_would_pass_31_bits_are_refused():
+    """A block walks up to 16 steps of 128 columns or 8 of 256, and a slice of K is rounded up to
+    128 elements for each of 32: the indexes behind the last one are 32-bit too."""
+    L = _lib.lib()
+    good = dict(struct_bytes=ctypes.sizeof(AdapterArgs), M=1, N=8, K=8, S=1, R=8, x_stride=8, y_stride=8,
+                out_stride=0x7fffff00, tile=4, dtype=_lib.DTYPE_BF16)
+    for bad in (dict(N=0x7fffff00), dict(N=0x7ffff000), dict(K=0x7fffff00), dict(K=0x7ffff800)):
+        args = AdapterArgs(**{**good, **bad})
+        assert L.actune_adapter_add(ctypes.byref(args), None) == _lib.ERR_INVALID_VALUE, bad
+    assert L.actune_adapter_workspace_size(1, 0x7fffff00, 1, 8, 4) == 0
+    assert L.actune_adapter_workspace_size(1, 0x7fff0000, 1, 8, 4) > 0
