@@ -451,7 +451,7 @@ __global__ void __launch_bounds__(AttnCfg<DP, NT>::WARPS * 32, 1)
     prefetch_tensormap(&tm_k);
     prefetch_tensormap(&tm_v);
   }
-  griddep_enter();
+  griddep_wait();
   if (warp == kProducer) {
     const AttnItem it = attn_item<BN, C::ROWS, MIXED>(p, lane, seqs);
     if (lane == 0) item_sh = it;
@@ -459,6 +459,9 @@ __global__ void __launch_bounds__(AttnCfg<DP, NT>::WARPS * 32, 1)
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
+  // Behind the allocation: a dependent that took the tensor memory first would wait for this
+  // launch to end, and this one for the memory.
+  griddep_launch_dependents();
   const uint32_t tmem = tmem_holder;
   const AttnItem it = item_sh;
   const int per_seq = p.T * p.rep;

@@ -170,3 +170,17 @@ def test_adapter_sizes_whose_last_step_would_pass_31_bits_are_refused():
         assert L.actune_adapter_add(ctypes.byref(args), None) == _lib.ERR_INVALID_VALUE, bad
     assert L.actune_adapter_workspace_size(1, 0x7fffff00, 1, 8, 4) == 0
     assert L.actune_adapter_workspace_size(1, 0x7fff0000, 1, 8, 4) > 0
+
+
+@pytest.mark.parametrize("source", ["prefix_attention.cu", "adapters.cu"])
+def test_dependents_are_let_in_behind_the_tensor_memory_allocation(source):
+    """A dependent launch may take an SM's tensor memory as soon as every block has signalled,
+    and then waits for this launch to end: a block that has not allocated by then never does."""
+    text = (ROOT / "actune_b200" / "csrc" / source).read_text()
+    kernels = [part for part in text.split("__global__")[1:] if "tmem_alloc(" in part]
+    assert kernels
+    for kernel in kernels:
+        kernel = re.sub(r"//.*", "", kernel)
+        signal = re.search(r"griddep_(enter|launch_dependents)\(", kernel).start()
+        allocated = kernel.index("tmem_alloc(")
+        assert allocated < signal and "__syncthreads();" in kernel[allocated:signal]
