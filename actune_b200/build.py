@@ -8,15 +8,20 @@ one shared library next to this file.  The CUDA runtime is linked statically so
 the library only needs the driver at run time.
 
 csrc/torch/*.cpp is host code against torch's headers: g++ compiles it into the CPython
-module _serving.so, which links the library above (found next to it).
+module _serving.so, which links the library above (found next to it).  It needs torch and a C++20
+compiler, and is built again for another torch; without torch, or with --library-only, the
+library alone is built, with nvcc alone.
 """
 from __future__ import annotations
 
 import argparse
 import concurrent.futures as cf
+import importlib.metadata
+import importlib.util
 import os
 import shutil
 import subprocess
+import sys
 import sysconfig
 from pathlib import Path
 
@@ -52,7 +57,7 @@ def _stale(target: Path, deps) -> bool:
 
 
 def build(force: bool = False, verbose_ptxas: bool = False, jobs: int | None = None,
-          out: Path | None = None) -> Path:
+          out: Path | None = None, library_only: bool = False) -> Path:
     headers = list(CSRC.glob("*.cuh")) + list(INCLUDE.glob("*.h"))
     srcs = sources()
     lib = Path(out) if out else LIB
@@ -83,15 +88,32 @@ def build(force: bool = False, verbose_ptxas: bool = False, jobs: int | None = N
         r = subprocess.run(cmd, capture_output=True, text=True)
         if r.returncode != 0:
             raise RuntimeError(f"nvcc link failed:\n{r.stdout}\n{r.stderr}")
-    if out is None:
-        build_torch_module(force)
+    if out is None and not library_only:
+        if torch_installed() is None:
+            print(f"torch is not installed: {TORCH_MODULE.name}, the serving operators' face to it, is not built",
+                  file=sys.stderr)
+        else:
+            build_torch_module(force)
     return lib
+
+
+def torch_installed() -> str | None:
+    """Version and place of the torch that a module built here is for; None without one."""
+    spec = importlib.util.find_spec("torch")
+    if spec is None:
+        return None
+    try:
+        return f"{importlib.metadata.version('torch')} at {spec.origin}"
+    except importlib.metadata.PackageNotFoundError:  # a source tree on the path
+        return spec.origin
 
 
 def build_torch_module(force: bool = False) -> Path:
     """Compile the CPython module of the serving operators (needs torch's headers and the
     built library)."""
-    if not force and not _stale(TORCH_MODULE, [TORCH_SOURCE, Path(__file__), *INCLUDE.glob("*.h")]):
+    built_for = BUILD / (TORCH_MODULE.stem + ".torch")
+    same = built_for.exists() and built_for.read_text() == torch_installed()
+    if not force and same and not _stale(TORCH_MODULE, [TORCH_SOURCE, Path(__file__), *INCLUDE.glob("*.h")]):
         return TORCH_MODULE
     import torch
     from torch.utils import cpp_extension
@@ -105,6 +127,7 @@ def build_torch_module(force: bool = False) -> Path:
     r = subprocess.run(cmd, capture_output=True, text=True)
     if r.returncode != 0:
         raise RuntimeError(f"g++ failed for {TORCH_SOURCE.name}:\n{r.stdout}\n{r.stderr}")
+    built_for.write_text(torch_installed())
     return TORCH_MODULE
 
 
@@ -114,8 +137,9 @@ def main():
     ap.add_argument("--verbose-ptxas", action="store_true")
     ap.add_argument("--jobs", type=int, default=None)
     ap.add_argument("--out", default=None, help="output library path (default: in-tree libactune_b200.so)")
+    ap.add_argument("--library-only", action="store_true", help="without torch's face of the serving operators")
     a = ap.parse_args()
-    print(build(force=a.force, verbose_ptxas=a.verbose_ptxas, jobs=a.jobs, out=a.out))
+    print(build(force=a.force, verbose_ptxas=a.verbose_ptxas, jobs=a.jobs, out=a.out, library_only=a.library_only))
 
 
 if __name__ == "__main__":
