@@ -188,3 +188,49 @@ def test_runs_on_the_current_stream_and_in_a_graph():
     static.copy_(x)
     graph.replay()
     assert all(torch.equal(a, b) for a, b in zip(out, want))
+
+
+# From 16 rows per SM on (2368 on 148 SMs) short rows take a warp each, long 16-bit ones
+# the kernel that streams them; the cases above of up to 1301 rows are below that.
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
+@pytest.mark.parametrize("bits,codes8", [(2, False), (2, True), (4, False), (4, True), (8, False)])
+def test_codes_of_many_rows(bits, codes8, dtype):
+    from actune_b200 import ops
+    for rows, width, groups in ((2400, 64, 1), (2500, 128, 5), (2400, 512, 2400), (2401, 576, 7), (2400, 1024, 16),
+                                (2600, 1088, 1), (2400, 2048, 100), (2400, 4096, 3), (2369, 8192, 1)):
+        x, residual, m = operands(rows, width, dtype, rows + width, gate="group", shift="group", groups=groups)
+        h, s, packed, scales = ops.gated_norm(x, residual, m["pre_weight"], post_weight=m["post_weight"],
+                                              gate=m["gate"], shift=m["shift"], quant_bits=bits, codes8=codes8)
+        plain, plain_s = ops.gated_norm(x, residual, m["pre_weight"], post_weight=m["post_weight"], gate=m["gate"],
+                                        shift=m["shift"])
+        want, want_scales = ops.quantize_group64(h, bits, codes8=codes8)
+        assert torch.equal(h, plain) and torch.equal(s, plain_s)
+        assert torch.equal(packed, want) and torch.equal(scales, want_scales), (rows, width)
+        ref_h, ref_s, tol_h, tol_s = expected(x, residual, m, 1.0, 1e-6, False)
+        check(s, ref_s, tol_s, dtype, "residual")
+        check(h, ref_h, tol_h, dtype, "norm")
+
+
+@pytest.mark.parametrize("gemma", [False, True])
+@pytest.mark.parametrize("post", [None, "width", "group"])
+@pytest.mark.parametrize("gate", [None, "width", "group"])
+@pytest.mark.parametrize("shift", [None, "group"])
+def test_modulations_of_many_rows(gemma, post, gate, shift):
+    for rows, groups, width, dtype in ((2480, 40, 129, torch.bfloat16), (2480, 1, 256, torch.bfloat16),
+                                       (2480, 62, 1024, torch.bfloat16), (2480, 2480, 2056, torch.float16),
+                                       (2480, 10, 640, torch.float32), (2480, 5, 4096, torch.float32)):
+        x, residual, m = operands(rows, width, dtype, 3 + groups, post=post, gate=gate, shift=shift, pre="group",
+                                  groups=groups)
+        run_and_check(x, residual, m, scale=1.3, gemma=gemma)
+
+
+@pytest.mark.parametrize("width", [256, 512, 1024, 2048, 4096])
+def test_a_row_of_nan_stays_alone_among_many(width):
+    from actune_b200 import ops
+    x, residual, m = operands(2600, width, torch.bfloat16, 11)
+    clean, clean_s = ops.gated_norm(x, residual, m["pre_weight"], post_weight=m["post_weight"])
+    x[7], x[9, 0], residual[1500, width - 1] = float("nan"), float("inf"), float("nan")
+    dirty, dirty_s = ops.gated_norm(x, residual, m["pre_weight"], post_weight=m["post_weight"])
+    keep = [i for i in range(2600) if i not in (7, 9, 1500)]
+    assert torch.equal(clean[keep], dirty[keep]) and torch.equal(clean_s[keep], dirty_s[keep])
+    assert dirty[7].isnan().all() and dirty[1500].isnan().all() and dirty_s[1500, 0].isfinite()
