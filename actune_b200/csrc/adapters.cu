@@ -38,7 +38,8 @@ __device__ __forceinline__ const int4* plan_tiles(const int32_t* plan) {
   return reinterpret_cast<const int4*>(plan + kHeader);
 }
 
-// One CTA.  Stable counting sort: 1024 rows at a time, the warps of a chunk one after
+// One CTA (800 rows 6 us, 6400 24 us, 38911 113 us, once for all the projections that a
+// batch passes through).  Stable counting sort: 1024 rows at a time, the warps of a chunk one after
 // the other, the lanes of a warp ranked among those of the same slot.
 __global__ void __launch_bounds__(1024) adapter_plan_kernel(const int32_t* __restrict__ slots, int M, int S, int tile,
                                                             int tiles_cap, int32_t* __restrict__ plan) {
@@ -892,9 +893,10 @@ int actune_adapter_add(const actune_adapter_args* a, void* stream) {
   CUtensorMap both[4] = {};
   const CUtensorMap* maps = nullptr;
   // Rows of `up` a multiple of 16 bytes, as tensor maps want them.  Low ranks with little to
-  // read and write are over sooner in 16-row parts, whose many small CTAs wait side by side:
-  // 800 rows 1024 -> 2560 at rank 16, 7.4 us and 10.9 us by tcgen05; 1024 rows 1024 -> 8192,
-  // 16.0 and 13.3 us; 1881 rows 312 -> 2560 at rank 64, 24.8 and 15.8 us.
+  // read and write are over as soon in 16-row parts, whose many small CTAs wait side by side:
+  // 16 x 50 rows 1024 -> 2560 at rank 16, 10.7 us and 11.2 us by tcgen05 (12 x 66 rows 10.3 and
+  // 9.7); 16 x 64 rows 1024 -> 8192, 21.5 and 16.8 us; 9 x 209 rows 312 -> 2560 at rank 64,
+  // 33.3 and 13.0 us (operands from memory).
   if (vec && a->tile == 128 && a->R % 8 == 0 && (a->R > 32 || a->M * a->N >= 4 << 20)) {
     p.split = a->workspace;
     p.factor = reinterpret_cast<float*>(a->workspace) + a->M * rp;

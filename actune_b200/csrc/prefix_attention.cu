@@ -37,12 +37,23 @@
 // exponent bits: its p, l and O carry a further 2^7 (p below 2^15), so that a long tail of
 // keys far below the maximum is weighed down to 2^-32 of it, not to 2^-25.
 //
+// p is rounded to the operands' 16 bits for the product with V (l sums the unrounded
+// ones), which adds about as much error as the rounding of the output itself: 2.2-2.3e-3
+// of its norm in bf16 where that alone is 1.7e-3, 2.6e-4 and 2.1e-4 in fp16.  p as two
+// 16-bit parts, in the place of the fp32 scores, brings that down to the output's rounding
+// for a second product and the splitting: 4 x 50 tokens 13.2 us for 11.8, 16 x 8 x 50 48.8
+// for 44.1, 32 single tokens behind 32768 57 for 50, 16 x 56 behind 2 histories 233 for
+// 159.  Not taken: it costs more than the bits that the output can hold are worth.
+//
 // Bounds: at head sizes up to 128 a block of 64 keys asks 128 rows x 64 exponentials of
 // each tile, as long as its products; with the softmax's latency between the two products
-// the main loop holds 65-70% of the measured matrix rate (75% at 256).  16 x 56 tokens, 32
-// heads of 128 behind 2 histories of up to 8192: 160 us where the tiles fit one wave, up to
-// 214 us where unevenly shared histories leave a second one; their products alone 41-55
-// us.  Small calls are launch, prologue and join: one sequence of 50 tokens 12 us.
+// the main loop holds 76% of the measured matrix rate at a head size of 256 (0.99 us a
+// block of keys for 128 rows), 64% at 128 (1.17 us for 256 rows), 44% at 64 (0.86 us);
+// launch, start and end of a CTA are 8 us beside that (148 tiles behind one prefix of 2048
+// to 8192).  16 x 56 tokens, 32 heads of 128 behind 2 histories of up to 8192: 159 us where
+// the tiles fit one wave, up to 214 us where unevenly shared histories leave a second one;
+// their products alone 41-55 us.  Small calls are launch, prologue and join: one sequence
+// of 50 tokens 11 us.
 #include "serving.cuh"
 
 namespace actune {

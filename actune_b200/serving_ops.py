@@ -114,10 +114,11 @@ def adapter_plan(slots, adapters):
     if not 1 <= adapters <= 8191:
         raise RuntimeError("between 1 and 8191 adapters")
     mean = rows / min(adapters, rows) if rows else 0
-    # The plan serves projections of every width, so its tiles are chosen by rows alone.  4
-    # against 16 rows: 32 adapters of 1 row, 4096 -> 22016, 11.6 and 15.5 us; of 3 rows, 1024
-    # -> 2560, 6.6 and 6.2 us.  16 against 128: 20 rows each, 4096 -> 12288, 18 and 30 us; 40
-    # rows, 2048 -> 32768 at rank 64, 92 and 55 us; 50 rows, 1024 -> 2560, 12.8 and 11.6 us.
+    # The plan serves projections of every width, so its tiles are chosen by rows alone
+    # (operands from memory, rank 16 where not said).  4 against 16 rows: 32 adapters of 1
+    # row, 4096 -> 22016, 15.4 and 22.0 us; of 3 rows, 1024 -> 2560, 7.5 and 7.3 us.  16
+    # against 128: 16 adapters of 20 rows, 4096 -> 12288, 18.4 and 21.4 us; of 40 rows, 2048
+    # -> 32768 at rank 64, 92 and 55 us; of 50 rows, 1024 -> 2560, 11.4 and 10.7 us.
     tile = 4 if mean <= 2 else 16 if mean <= 32 else 128
     size = _lib.lib().actune_adapter_plan_size(rows, adapters, tile)
     if size == 0:
@@ -133,8 +134,10 @@ def adapter_add(y, x, down, up, scale, plan, *, out=None):
 
     down [S, R, K], up [S, N, R] (1 <= R <= 128) and x, y in one dtype, float16 or
     bfloat16; scale float32 [S]; ``plan`` from ``adapter_plan``.  Rows of x, y and out
-    may be strided; ``out=y`` adds in place.  Sums are kept in 32 bits from x to the one
-    rounding of out."""
+    may be strided; ``out=y`` adds in place, and ``out`` overlaps no other operand.  Both
+    products are summed in 32 bits and out is rounded once; between them ``down x`` is held
+    in 32 bits in tiles of 4 rows, and in two 16-bit parts (16 bits of significand in
+    bfloat16, 22 in float16) where matrix instructions take it."""
     return _checked(_serving().adapter_add(y, x, down, up, scale, plan.buffer, plan.rows, plan.adapters, plan.tile,
                                            out), "adapter_add")
 
@@ -156,9 +159,16 @@ def shared_prefix_attention(q, prefix_k, prefix_v, k, v, *, starts=None, prefix_
     j <= lens[b] - T + t, without it all of them.  A query that sees nothing gets zeros.
     ``scale`` (positive) defaults to D ** -0.5.
 
+    Scores, softmax and sums are held in 32 bits; the probabilities are rounded to the
+    operands' type for their product with the values, which adds about as much error as the
+    rounding of the output (the scalar kernel keeps them in 32 bits).  A value that is not
+    finite may reach queries of its own sequence that ``causal`` keeps from it, and reaches
+    no other sequence.
+
     float16 or bfloat16, D <= 256 contiguous, any other strides: cache views such as
     cache[:, :, 0].unsqueeze(2) and slices of a fused projection need no copy.  With D a
     multiple of 8 and 16-byte aligned rows it runs on the tensor cores, otherwise on a
-    scalar kernel many times slower.  Returns [B, T, H, D], contiguous."""
+    scalar kernel many times slower (4 x 50 tokens, 8 heads of 64: 11 and 123 us).  Returns
+    [B, T, H, D], contiguous; ``out`` gives the room for it and overlaps no input."""
     return _checked(_serving().shared_prefix_attention(q, prefix_k, prefix_v, k, v, starts, prefix_lens, lens, causal,
                                                        scale, out), "shared_prefix_attention")

@@ -65,9 +65,12 @@ int actune_gated_norm(const actune_gated_norm_args* args, void* stream);
  *
  * actune_adapter_add: x [M, K], y and out [M, N], down [S, R, K], up [S, N, R], all of
  * `dtype` (F16 or BF16), 1 <= R <= 128; scale float [S]; x, y and out have row strides;
- * out may be y itself (same pointer and stride), and overlaps nothing else.  The sums
- * down x are kept in fp32 in the workspace (16-byte aligned, at least
- * actune_adapter_workspace_size bytes); the result is rounded once.  Any K, N, R and
+ * out may be y itself (same pointer and stride), and overlaps nothing else.  down x
+ * is summed in fp32 and goes through the workspace (16-byte aligned, at least
+ * actune_adapter_workspace_size bytes).  Where the second product is one of matrix
+ * instructions (all but tiles of 4 in the vector form with R <= 64 a multiple of 8) it enters
+ * it as two parts of `dtype`: 16 bits of significand in bf16, 22 in fp16.  up (down x) is
+ * summed in fp32, and the result is rounded once.  Any K, N, R and
  * alignment; 16-byte aligned operands with K, N and the strides multiples of 8 and R a
  * multiple of 4 run the vector form. */
 size_t actune_adapter_plan_size(int64_t M, int64_t S, int tile);
@@ -105,8 +108,10 @@ int actune_adapter_add(const actune_adapter_args* args, void* stream);
  * clamped).  All three are read on the device.
  * q [B, T, H, D], prefix_k and prefix_v [G, P, KV, D], k and v [B, S, KV, D], D <= 256,
  * of `dtype` (F16 or BF16), with D contiguous and the given strides; out [B, T, H, D]
- * contiguous.  Scores, softmax and sums are fp32; p is rounded to `dtype` for the
- * product with V, as the tensor core takes it.
+ * contiguous, overlapping no input.  Scores, softmax and sums are fp32; p is rounded to
+ * `dtype` for the product with V, as the tensor core takes it.  A value of v that is not
+ * finite may reach queries of its own sequence that causal keeps from it, and reaches no
+ * other sequence.
  * workspace: at least actune_prefix_attention_workspace_size bytes, 16-byte aligned.
  * Operands with D a multiple of 8, 16-byte aligned, and strides that are positive
  * multiples of 8 run on the tensor cores; others on a scalar kernel. */
