@@ -19,6 +19,7 @@ from __future__ import annotations
 from dataclasses import dataclass
 
 import torch
+from torch.utils import _pytree as pytree
 
 from . import _lib
 
@@ -93,6 +94,13 @@ class AdapterPlan:
                                                       torch.cuda.current_stream(slots.device).cuda_stream),
                        "adapter_plan")
         return self
+
+
+# Among the arguments of a GraphReplay call a plan is its buffer, copied like any tensor,
+# and its sizes, which are part of the call's identity.
+pytree.register_pytree_node(AdapterPlan, lambda p: ([p.buffer], (p.rows, p.adapters, p.tile)),
+                            lambda leaves, sizes: AdapterPlan(*leaves, *sizes),
+                            serialized_type_name="actune_b200.AdapterPlan")
 
 
 def _check_slots(slots):

@@ -165,3 +165,22 @@ def test_adapters_are_refused_where_a_gradient_would_pass_them_by():
             layer(x.clone().requires_grad_())
         with pytest.raises(RuntimeError, match="CUDA required"):
             layer(x)
+
+
+def test_a_plan_among_the_arguments_is_an_input_too():
+    class ArgumentReplay(GraphReplay):
+        def _record(self, slot, tree):
+            (_, plan), _ = torch.utils._pytree.tree_unflatten(slot.statics, tree)
+            output = []
+            graph = types.SimpleNamespace(replay=lambda: output.__setitem__(slice(None), plan.buffer.tolist()))
+            return _Capture(graph, output, {})
+
+    replay = ArgumentReplay(lambda x, plan: x, {})
+    replay.enabled = True
+    x, slots = torch.zeros(2, 3), list(range(2000))  # longer than a tensor's repr shows
+    for first in (0, 5, 7):
+        slots[1000] = first
+        assert replay(x, plan_of(slots)) == slots
+    assert len(replay.graphs) == 1
+    replay(x, plan_of(slots, tile=128))
+    assert len(replay.graphs) == 2
