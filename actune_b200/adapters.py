@@ -14,10 +14,11 @@ runs in:
         model(x)
 
 Outside a scope the projections run alone.  ``GraphReplay`` takes the active plan (and
-one among its arguments) as an input: calls under plans of the same sizes replay one graph, each with its own routing,
-and a call outside a scope replays another.  A CUDA graph captured by other means reads
-the buffer of the plan it was captured under: keep that plan as long as the graph;
-``plan.update(slots)`` before a replay routes the same number of rows anew.
+one among its arguments) as an input: calls under plans of the same sizes replay one
+graph, each with its own routing, and a call outside a scope replays another.  A CUDA
+graph captured by other means reads the buffer of the plan it was captured under: keep
+that plan as long as the graph; ``plan.update(slots)`` before a replay routes the same
+number of rows anew.
 """
 from __future__ import annotations
 

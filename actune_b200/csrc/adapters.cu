@@ -39,8 +39,8 @@ __device__ __forceinline__ const int4* plan_tiles(const int32_t* plan) {
 }
 
 // One CTA (800 rows 6 us, 6400 24 us, 38911 113 us, once for all the projections that a
-// batch passes through).  Stable counting sort: 1024 rows at a time, the warps of a chunk one after
-// the other, the lanes of a warp ranked among those of the same slot.
+// batch passes through).  Stable counting sort: 1024 rows at a time, the warps of a chunk
+// one after the other, the lanes of a warp ranked among those of the same slot.
 __global__ void __launch_bounds__(1024) adapter_plan_kernel(const int32_t* __restrict__ slots, int M, int S, int tile,
                                                             int tiles_cap, int32_t* __restrict__ plan) {
   extern __shared__ int32_t sh[];  // per slot (S + 1: the last is "none"): count, then next place
